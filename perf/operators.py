@@ -27,29 +27,29 @@ MIN_EXPONENT = -64  # of a page's scale
 def listed():
     return [
         # One decoding step of a full server: every request adds a token, one in sixteen needs a page.
-        dict(name="tables, a step of 256", op="tables", requests=256, cached=8192, added=1, page=16, short=False),
+        dict(name="tables: a step of 256", op="tables", requests=256, cached=8192, added=1, page=16, short=False),
         # Prompts admitted together behind a shared prefix; ragged, thousands of new pages.
-        dict(name="tables, 48 prompts", op="tables", requests=48, cached=2048, added=4096, page=64, short=False),
+        dict(name="tables: 48 prompts", op="tables", requests=48, cached=2048, added=4096, page=64, short=False),
         # The same decoding step's keys and values: one token a request, into pages that are partly full.
-        dict(name="write, a step of 256", op="write", requests=256, added=1, kv_heads=8, dim=128, page=16, type="bf16"),
+        dict(name="write: a step of 256", op="write", requests=256, added=1, kv_heads=8, dim=128, page=16, type="bf16"),
         # Prompts' keys and values: whole pages, first and last ones partial.
-        dict(name="write, 8 prompts", op="write", requests=8, added=4096, kv_heads=8, dim=64, page=64, type="f16"),
+        dict(name="write: 8 prompts", op="write", requests=8, added=4096, kv_heads=8, dim=64, page=64, type="f16"),
         # The smallest call: one user, a short context; latency.
-        dict(name="attention, one request", op="attention", requests=1, length=700, queries=1, q_heads=32, kv_heads=8, dim=128, page=16, type="bf16"),
+        dict(name="attention: one request", op="attention", requests=1, length=700, queries=1, q_heads=32, kv_heads=8, dim=128, page=16, type="bf16"),
         # An ordinary batch of decoding requests, ragged.
-        dict(name="attention, 64 requests", op="attention", requests=64, length=8192, queries=1, q_heads=32, kv_heads=8, dim=128, page=64, type="bf16"),
+        dict(name="attention: 64 requests", op="attention", requests=64, length=8192, queries=1, q_heads=32, kv_heads=8, dim=128, page=64, type="bf16"),
         # Few requests with very long contexts: the work has to be split along the keys.
-        dict(name="attention, 3 long contexts", op="attention", requests=3, length=262144, queries=1, q_heads=64, kv_heads=8, dim=128, page=128, type="f16"),
+        dict(name="attention: 3 long contexts", op="attention", requests=3, length=262144, queries=1, q_heads=64, kv_heads=8, dim=128, page=128, type="f16"),
         # Drafted tokens checked together, a head of keys for each head of queries, wide heads.
-        dict(name="attention, 32 drafts", op="attention", requests=32, length=2500, queries=5, q_heads=16, kv_heads=16, dim=256, page=16, type="f16"),
+        dict(name="attention: 32 drafts", op="attention", requests=32, length=2500, queries=5, q_heads=16, kv_heads=16, dim=256, page=16, type="f16"),
         # Pieces of prompts against what the cache holds of them: bound by arithmetic.
-        dict(name="attention, 6 prompt pieces", op="attention", requests=6, length=6000, queries=509, q_heads=16, kv_heads=4, dim=64, page=32, type="bf16"),
+        dict(name="attention: 6 prompt pieces", op="attention", requests=6, length=6000, queries=509, q_heads=16, kv_heads=4, dim=64, page=32, type="bf16"),
         # One token through a square projection: latency.
-        dict(name="matvec, 1 x 4096 x 4096", op="matvec", rows=1, n=4096, k=4096, group=128, zeros=False, type="bf16"),
+        dict(name="matvec: 1 x 4096 x 4096", op="matvec", rows=1, n=4096, k=4096, group=128, zeros=False, type="bf16"),
         # A small batch, an odd number of outputs, zero points.
-        dict(name="matvec, 13 x 10001 x 8192", op="matvec", rows=13, n=10001, k=8192, group=64, zeros=True, type="f16"),
+        dict(name="matvec: 13 x 10001 x 8192", op="matvec", rows=13, n=10001, k=8192, group=64, zeros=True, type="f16"),
         # One token through a large feed-forward projection: the weights' 4 bits are all there is.
-        dict(name="matvec, 1 x 28672 x 8192", op="matvec", rows=1, n=28672, k=8192, group=128, zeros=True, type="bf16"),
+        dict(name="matvec: 1 x 28672 x 8192", op="matvec", rows=1, n=28672, k=8192, group=128, zeros=True, type="bf16"),
     ]
 
 
