@@ -74,6 +74,10 @@ def _load():
         pipes.gern_qk_softmax_run_no_alloc.argtypes = [vp, vp, vp, vp, i64, i64, C.c_float, vp]
     pipes.gern_gemm_schedule_create.argtypes = [C.c_int, C.c_int, C.POINTER(vp)]
     pipes.gern_gemm_schedule_run.argtypes = [vp, vp, vp, vp, vp]
+    pipes.gern_page_table_create.argtypes = [i64, C.c_int, C.POINTER(vp)]
+    pipes.gern_page_table_run.argtypes = [vp, vp, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp]
+    pipes.gern_cache_write_create.argtypes = [i64, i64, C.c_int, C.c_int, C.POINTER(vp)]
+    pipes.gern_cache_write_run.argtypes = [vp, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, i64, vp]
     cpp = C.POINTER(C.c_char_p)
     hip.gern_hip_compile.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(vp)]
     hip.gern_hip_compile_only.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(sz)]
@@ -292,3 +296,118 @@ class QKSoftmax(_Pipeline):
         run = pipelines_lib().gern_qk_softmax_run_no_alloc if no_alloc else pipelines_lib().gern_qk_softmax_run
         _check(run(self.h, _ptr(Q), _ptr(K), _ptr(S), M, N, float(scale), stream))
         return S
+
+
+_TYPES = {"bf16": 0, "f16": 1}
+
+
+def _type(dtype):
+    if dtype not in _TYPES:
+        raise GernError("dtype must be \"bf16\" or \"f16\", not %r" % (dtype,))
+    return _TYPES[dtype]
+
+
+def _expect(ok, what):
+    if not ok:
+        raise GernError(what)
+
+
+class _ServingPipeline(_Pipeline):
+    """A pipeline of torch tensors: it checks types, layouts and devices before it hands addresses to the C ABI."""
+
+    def __init__(self):
+        super().__init__()
+        import torch
+        self._torch = torch
+        self._int32_type = torch.int32
+        self._device = torch.cuda.current_device() if torch.cuda.is_available() else None
+
+    def _on_gpu(self, *tensors):
+        """All on the GPU that the pipeline was created on, which is the current one (a kernel runs where its code was loaded)."""
+        for t in tensors:
+            if not t.is_cuda or t.get_device() != self._device:
+                raise GernError("every tensor must be on the pipeline's GPU (%s), not on %s" % (self._device, t.device))
+        if self._torch.cuda.current_device() != self._device:
+            raise GernError("the pipeline's GPU (%s) must be the current one" % self._device)
+
+    def _int32(self, **tensors):
+        for name, t in tensors.items():
+            if t.dtype is not self._int32_type or not t.is_contiguous():
+                raise GernError(name + " must be a contiguous int32 tensor")
+
+    def _halves(self, **tensors):
+        """16-bit floats of the pipeline's type, contiguous but for the stride of their first dimension."""
+        want = self._torch.bfloat16 if self.dtype == "bf16" else self._torch.float16
+        for name, t in tensors.items():
+            if t.dtype is not want:
+                raise GernError("%s must be %s" % (name, self.dtype))
+            inner = 1
+            for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+                if stride != inner and size != 1:
+                    raise GernError(name + " must be contiguous in all but its first dimension")
+                inner *= size
+
+    def _cache(self, k_cache, v_cache, k_scales, v_scales):
+        """(pages, heads) of a paged cache."""
+        torch, shape = self._torch, k_cache.shape
+        if len(shape) != 4 or shape[2] != self.page_size or shape[3] != self.head_dim or v_cache.shape != shape:
+            raise GernError("the cache's codes must be [pages, heads, page_size = %d, head_dim = %d]" % (self.page_size, self.head_dim))
+        if k_scales.shape != shape[:2] or v_scales.shape != shape[:2]:
+            raise GernError("the cache's scales must be [pages, heads]")
+        for t in (k_cache, v_cache):
+            if t.dtype not in (torch.float8_e4m3fn, torch.uint8) or not t.is_contiguous():
+                raise GernError("the cache's codes must be contiguous float8_e4m3fn (or uint8)")
+        for t in (k_scales, v_scales):
+            if t.dtype is not torch.float32 or not t.is_contiguous():
+                raise GernError("the cache's scales must be contiguous float32")
+        return shape[0], shape[1]
+
+
+def _pitch(t):
+    """Elements from one entry of the first dimension to the next."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t[0].numel() if t.shape[0] else 0)
+
+
+class PageTable(_ServingPipeline):
+    """Block tables and slot maps of a batch of requests (gern_page_table_run)."""
+
+    def __init__(self, page_size=16, flags=0):
+        super().__init__()
+        self.page_size = page_size
+        _check(pipelines_lib().gern_page_table_create(page_size, flags, C.byref(self.h)))
+
+    def __call__(self, cached, added, free_pages, free_count, table, lengths, starts, slots, counts, stream=None):
+        """cached, added [requests], free_pages [any], free_count [1] in; table [requests, width] (new entries only),
+        lengths [requests], starts [requests + 1], slots [tokens], counts [2] (pages left, pages missing) out; int32."""
+        self._int32(cached=cached, added=added, free_pages=free_pages, free_count=free_count, table=table, lengths=lengths, starts=starts, slots=slots,
+                    counts=counts)
+        n = cached.shape[0]
+        _expect(tuple(cached.shape) == tuple(added.shape) == tuple(lengths.shape) == (n,) and tuple(starts.shape) == (n + 1,) and table.dim() == 2 and
+                table.shape[0] == n and free_pages.dim() == slots.dim() == 1 and free_count.numel() == 1 and counts.numel() == 2,
+                "cached, added and lengths must be [requests], starts [requests + 1], table [requests, width], free_count [1] and counts [2]")
+        self._on_gpu(cached, added, free_pages, free_count, table, lengths, starts, slots, counts)
+        _check(pipelines_lib().gern_page_table_run(self.h, _ptr(cached), _ptr(added), n, _ptr(free_pages), free_pages.shape[0], _ptr(free_count),
+                                                   _ptr(table), table.shape[1], _ptr(lengths), _ptr(starts), _ptr(slots), slots.shape[0], _ptr(counts),
+                                                   stream))
+        return table, slots
+
+
+class CacheWrite(_ServingPipeline):
+    """New keys and values into a paged cache in 8 bits (gern_cache_write_run)."""
+
+    def __init__(self, head_dim=128, page_size=16, dtype="bf16", flags=0):
+        super().__init__()
+        self.head_dim, self.page_size, self.dtype = head_dim, page_size, dtype
+        _check(pipelines_lib().gern_cache_write_create(head_dim, page_size, _type(dtype), flags, C.byref(self.h)))
+
+    def __call__(self, k, v, slots, k_cache, v_cache, k_scales, v_scales, stream=None):
+        """k, v [tokens, heads, head_dim] (any stride from token to token); slots [tokens] int32, -1 = not stored; the
+        cache [pages, heads, page_size, head_dim] float8_e4m3fn with scales [pages, heads] float32 is updated."""
+        pages, heads = self._cache(k_cache, v_cache, k_scales, v_scales)
+        n = slots.shape[0]
+        self._int32(slots=slots)
+        self._halves(k=k, v=v)
+        _expect(tuple(k.shape) == tuple(v.shape) == (n, heads, self.head_dim), "k and v must be [tokens, heads, head_dim]")
+        self._on_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
+        _check(pipelines_lib().gern_cache_write_run(self.h, _ptr(k), _pitch(k), _ptr(v), _pitch(v), _ptr(slots), n, heads, _ptr(k_cache), _ptr(v_cache),
+                                                    _ptr(k_scales), _ptr(v_scales), pages, stream))

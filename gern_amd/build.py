@@ -23,6 +23,8 @@ CXXFLAGS = ["-std=c++20", "-O2", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_
 HIPFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang",
             "-packed-fp32-ops", "-I" + HERE]
 
+PIPELINE_SOURCES = [os.path.join(HERE, "csrc", n) for n in ("pipelines.cpp", "serving_pipelines.cpp")]
+
 
 def run(cmd):
     print("+ " + " ".join(cmd), flush=True)
@@ -41,8 +43,8 @@ def build_native():
     no_alloc = os.path.join(HERE, "csrc", "qk_no_alloc.o")
     run([os.path.join(ROCM, "bin", "hipcc")] + HIPFLAGS + ["-fPIC", "-I" + os.path.join(ROOT, "include"), "-c",
                                                           os.path.join(HERE, "csrc", "qk_no_alloc.hip"), "-o", no_alloc])
-    run(["g++"] + CXXFLAGS + ["-shared", os.path.join(HERE, "csrc", "pipelines.cpp"), no_alloc, "-L" + HERE, "-lgern",
-                               "-lgern_hip", "-L" + os.path.join(ROCM, "lib"), "-lamdhip64", "-ldl", rpath, "-o",
+    run(["g++"] + CXXFLAGS + ["-shared"] + PIPELINE_SOURCES + [no_alloc, "-L" + HERE, "-lgern", "-lgern_hip",
+                               "-L" + os.path.join(ROCM, "lib"), "-lamdhip64", "-ldl", rpath, "-o",
                                os.path.join(HERE, "libgern_pipelines.so")])
 
 
@@ -99,7 +101,7 @@ def sanitize_check():
                             "-lamdhip64", "-lhiprtc", rpath, "-o", os.path.join(out, "libgern_hip.so")])
     srcs = sorted(glob.glob(os.path.join(HERE, "src", "*.cpp")))
     run(["g++"] + flags + ["-shared"] + srcs + ["-L" + out, "-lgern_hip", "-ldl", rpath, "-o", os.path.join(out, "libgern.so")])
-    run(["g++"] + flags + ["-shared", os.path.join(HERE, "csrc", "pipelines.cpp"), "-L" + out, "-lgern", "-lgern_hip", "-ldl",
+    run(["g++"] + flags + ["-shared"] + PIPELINE_SOURCES + ["-L" + out, "-lgern", "-lgern_hip", "-ldl",
                             rpath, "-o", os.path.join(out, "libgern_pipelines.so")])
     tdir = os.path.join(ROOT, "tests", "cpp")
     programs = []

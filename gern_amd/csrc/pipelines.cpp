@@ -4,6 +4,8 @@
 // evaluate with the caller's buffers.
 #include "gern_pipelines.h"
 
+#include "pipeline.h"
+
 #include "annot/blur.h"
 #include "annot/lds_matrix.h"
 #include "annot/mm.h"
@@ -30,10 +32,31 @@ namespace {
 
 thread_local std::string g_error;
 
-int fail(const std::string &msg) {
+}  // namespace
+
+int gern_detail::fail(const std::string &msg) {
     g_error = msg;
     return 1;
 }
+
+int gern_detail::failHip(const std::string &who) {
+    std::string msg(gern_hip_last_error(nullptr, 0) + 1, '\0');
+    gern_hip_last_error(msg.data(), msg.size());
+    msg.resize(msg.size() - 1);
+    return fail(who + ": " + msg);
+}
+
+// GERN_EXPERIMENTS=1, see pipeline.h
+bool gern_detail::experiments() {
+    const char *v = std::getenv("GERN_EXPERIMENTS");
+    return v != nullptr && std::string(v) == "1";
+}
+
+using gern_detail::experiments;
+using gern_detail::fail;
+using gern_detail::finish;
+
+namespace {
 
 // Directory that holds this library; the gernel headers live next to it.
 // Where gernels/ and annot/ are: the directory of this library, unless
@@ -53,46 +76,11 @@ std::string packageDir() {
     return ".";
 }
 
-// GERN_EXPERIMENTS=1 lets the environment change what the pipelines are built from (extra compiler
-// options, other band heights and wavefront counts): for measurements, never needed for results.
-bool experiments() {
-    const char *v = std::getenv("GERN_EXPERIMENTS");
-    return v != nullptr && std::string(v) == "1";
-}
-
 AbstractDataTypePtr f32(const std::string &name, annot::MatrixF32::Role role) {
     return AbstractDataTypePtr(new const annot::MatrixF32(name, role));
 }
 
 }  // namespace
-
-struct gern_pipeline_s {
-    enum Kind { BLUR, SOFTMAX, GEMM_F32, GEMM_BF16, QK_SOFTMAX, GEMM_SCHEDULE } kind;
-    std::unique_ptr<Runner> runner;  // null in compile-only mode
-    std::unique_ptr<Runner> exact;   // GEMM: the direct-to-LDS matrix-core kernel (rows of A in whole 16-byte pieces)
-    std::unique_ptr<Runner> tail;    // fp32 GEMM in overwrite mode: C += of the last K % 4 columns
-    bool accumulate = true;          // GEMM: C += A * B (false: C = A * B)
-    int create_flags = 0;
-    std::string source;
-    std::string kernel_name;
-    std::string exact_source, exact_kernel_name;
-    bool last_run_exact = false;
-    // blur
-    int64_t nx = 0, ny = 0, stride = 0;
-    // softmax / qk
-    int64_t ncol = 0;
-    int64_t head_dim = 0;
-    // qk on 256 x 256 tiles: the memory through which the workgroups of a row block exchange row statistics
-    bool qk_tiles = false;
-    void *qk_scratch = nullptr;
-    // the exchange memory of the library (csrc/qk_no_alloc.hip) on this pipeline's GPU; null if it has none
-    void *qk_shared_scratch = nullptr;
-    bool qk_used_shared = false;      // a run went through qk_shared_scratch since the last gern_pipeline_faults
-    bool qk_default_period = true;    // built with the tag period every user of the shared memory agrees on
-    void *last_stream = nullptr;
-    // parameter names
-    std::vector<std::string> names;
-};
 
 namespace {
 
@@ -101,8 +89,10 @@ int64_t qkWaves(int64_t n) {
     return (n >= 2048 && n % 512 == 0) ? 8 : 4;
 }
 
+}  // namespace
+
 // Generates (and, unless compile-only, loads) the program.
-int finish(gern_pipeline_s *p, Composable program, int flags, int min_waves_per_simd = 0, int xcd_band_rows = 0) {
+int gern_detail::finish(gern_pipeline_s *p, Composable program, int flags, int min_waves_per_simd, int xcd_band_rows) {
     std::string include = "-I " + packageDir();
     if (const char *extra = std::getenv("GERN_PIPELINE_EXTRA_OPTIONS"); extra != nullptr && experiments()) {
         include += std::string(" ") + extra;  // e.g. "-DNAME=value"
@@ -157,8 +147,6 @@ int finish(gern_pipeline_s *p, Composable program, int flags, int min_waves_per_
         return fail(e.what());
     }
 }
-
-}  // namespace
 
 // csrc/qk_no_alloc.hip: the address of the library's exchange memory on the current GPU (looked up, once per
 // GPU, on the first call).  Weak: a build of this file without that object has no such memory.
@@ -765,6 +753,14 @@ int gern_pipeline_faults(gern_pipeline p, int64_t *count) {
     } catch (const std::exception &e) {
         return fail(e.what());
     }
+    if (p->fault_count != nullptr) {
+        uint32_t faults = 0;
+        if (gern_hip_sync() != 0 || gern_hip_memcpy_d2h(&faults, p->fault_count, sizeof(faults)) != 0 ||
+            (faults != 0 && gern_hip_memset(p->fault_count, 0, sizeof(faults)) != 0)) {
+            return gern_detail::failHip("gern_pipeline_faults");
+        }
+        *count += (int64_t)faults;
+    }
     if (!p->qk_tiles || !p->runner) {
         return 0;
     }
@@ -935,12 +931,18 @@ const char *gern_pipeline_source(gern_pipeline p) {
     if (p == nullptr) {
         return "";
     }
+    if (!p->variants.empty()) {
+        return p->variants[p->last_variant].source.c_str();
+    }
     return p->last_run_exact && !p->exact_source.empty() ? p->exact_source.c_str() : p->source.c_str();
 }
 
 const char *gern_pipeline_kernel_name(gern_pipeline p) {
     if (p == nullptr) {
         return "";
+    }
+    if (!p->variants.empty()) {
+        return p->variants[p->last_variant].kernel_name.c_str();
     }
     if (p->kernel_name.empty() && p->runner) {
         p->kernel_name = p->runner->getKernelName();
@@ -959,8 +961,15 @@ int gern_pipeline_destroy(gern_pipeline p) {
                 r->release();
             }
         }
-        if (p->qk_scratch != nullptr) {
-            gern_hip_free(p->qk_scratch);
+        for (auto &v : p->variants) {
+            if (v.runner) {
+                v.runner->release();
+            }
+        }
+        for (void *memory : {p->qk_scratch, static_cast<void *>(p->fault_count)}) {
+            if (memory != nullptr) {
+                gern_hip_free(memory);
+            }
         }
     }
     delete p;

@@ -1,0 +1,313 @@
+// C ABI over the operators of a serving step (include/gern_pipelines.h): block
+// tables, the paged 8-bit cache of keys and values, attention over it, and
+// products with 4-bit weights.  Like the other pipelines these are programs
+// against Gern's C++ API; each launch is one gernel whose pieces are tiled over
+// the grid.
+#include "pipeline.h"
+
+#include "annot/paged_cache.h"
+#include "gern_hip.h"
+
+#include <algorithm>
+#include <cstdint>
+
+using namespace gern;
+using gern_detail::fail;
+using gern_detail::failHip;
+using gern_detail::finish;
+
+namespace {
+
+// A pipeline under construction: destroyed unless it is handed out.
+class Draft {
+public:
+    Draft(gern_pipeline_s::Kind kind, int flags) : p(new gern_pipeline_s{}), compile_only((flags & GERN_PIPELINE_COMPILE_ONLY) != 0) {
+        p->kind = kind;
+        p->create_flags = flags;
+    }
+    ~Draft() {
+        if (p != nullptr) {
+            gern_pipeline_destroy(p);
+        }
+    }
+    Draft(const Draft &) = delete;
+    Draft &operator=(const Draft &) = delete;
+    gern_pipeline_s *operator->() {
+        return p;
+    }
+    // Compiles one more program of the pipeline.
+    int add(Composable program, int flags) {
+        gern_pipeline_s one{};
+        const int rc = finish(&one, program, flags);
+        if (rc == 0) {
+            const std::string name = one.runner ? one.runner->getKernelName() : one.kernel_name;
+            p->variants.push_back({std::move(one.runner), one.source, name});
+        }
+        return rc;
+    }
+    // The device word that gern_pipeline_faults reads.
+    int addFaultCount(const char *who) {
+        void *word = nullptr;
+        if (compile_only) {
+            return 0;
+        }
+        if (gern_hip_malloc(&word, sizeof(uint32_t)) != 0 || gern_hip_memset(word, 0, sizeof(uint32_t)) != 0) {
+            if (word != nullptr) {
+                gern_hip_free(word);
+            }
+            return failHip(who);
+        }
+        p->fault_count = static_cast<uint32_t *>(word);
+        return 0;
+    }
+    gern_pipeline handOut() {
+        gern_pipeline_s *done = p;
+        p = nullptr;
+        return done;
+    }
+
+private:
+    gern_pipeline_s *p;
+    bool compile_only;
+};
+
+bool usable(gern_pipeline p, gern_pipeline_s::Kind kind) {
+    return p != nullptr && p->kind == kind;
+}
+
+int evaluate(gern_pipeline p, size_t variant, const char *who, void *stream, const std::map<std::string, void *> &args) {
+    try {
+        Runner *runner = p->variants[variant].runner.get();
+        if (runner == nullptr) {
+            return fail(std::string(who) + ": the pipeline was created compile-only");
+        }
+        runner->setStream(stream);
+        runner->evaluate(args);
+        p->last_variant = variant;
+    } catch (const std::exception &e) {
+        return fail(e.what());
+    }
+    return 0;
+}
+
+bool aligned(const void *pointer, uintptr_t bytes) {
+    return reinterpret_cast<uintptr_t>(pointer) % bytes == 0;
+}
+
+// Whether [a, a + na) and [b, b + nb), sizes in bytes, share memory.
+bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+    return na > 0 && nb > 0 && pa < pb + (uintptr_t)nb && pb < pa + (uintptr_t)na;
+}
+
+bool goodPageSize(int64_t page_size) {
+    return page_size >= 16 && page_size <= 128 && (page_size & (page_size - 1)) == 0;
+}
+
+bool goodHeadDim(int64_t head_dim) {
+    return head_dim >= 64 && head_dim <= 256 && head_dim % 64 == 0;
+}
+
+bool goodType(int type) {
+    return type == GERN_TYPE_BF16 || type == GERN_TYPE_F16;
+}
+
+std::string typeName(int type) {
+    return type == GERN_TYPE_BF16 ? "gernels::Bf16" : "gernels::F16";
+}
+
+// A name's Variable bound to a value, for PieceFunction's constants.
+std::pair<const std::string, Variable> constant(const std::string &name, int64_t value) {
+    return {name, Variable(name).bind(value)};
+}
+
+}  // namespace
+
+extern "C" {
+
+// --------------------------------------------------------------------------------------------- block tables
+
+// Most requests a workgroup of 1024 threads takes the prefix sums of: eight a thread.
+static_assert(GERN_PAGE_TABLE_MAX_REQUESTS == 8 * 1024, "the variants of gern_page_table_create");
+
+int gern_page_table_create(int64_t page_size, int flags, gern_pipeline *out) {
+    if (out == nullptr) {
+        return fail("gern_page_table_create: null argument");
+    }
+    *out = nullptr;
+    if (!goodPageSize(page_size)) {
+        return fail("gern_page_table_create: page_size must be 16, 32, 64 or 128");
+    }
+    try {
+        Draft p(gern_pipeline_s::PAGE_TABLE, flags);
+        p->page_size = page_size;
+        for (int64_t per : {1, 8}) {
+            AbstractDataTypePtr batch(new const annot::WholeADT("batch", "gernels::RequestLengths"));
+            AbstractDataTypePtr free_pages(new const annot::WholeADT("free_pages", "gernels::FreePages"));
+            AbstractDataTypePtr table(
+                new const annot::PiecesADT<hip::PageTableOut>("table", "gernels::PageTableOut", "share", {{"shares", &hip::PageTableOut::shares}}));
+            annot::PieceFunction extend("gernels::extend_page_table", "gernels/page_table.h", {batch, free_pages}, table, {"shares"},
+                                        {"page", "threads", "per"});
+            Variable one("one"), threads("block");
+            Composable program = Global((Tile(table["shares"], one.bind(1)) || Grid::BLOCK_X)(
+                                            extend[{constant("page", page_size), constant("threads", 1024), constant("per", per)}](batch, free_pages, table)),
+                                        {{Grid::BLOCK_DIM_X, threads.bind(1024)}});
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                return 1;
+            }
+        }
+        *out = p.handOut();
+    } catch (const std::exception &e) {
+        return fail(e.what());
+    }
+    return 0;
+}
+
+int gern_page_table_run(gern_pipeline p, const int32_t *cached, const int32_t *added, int64_t requests, const int32_t *free_pages,
+                        int64_t free_capacity, const int32_t *free_count, int32_t *table, int64_t table_width, int32_t *lengths,
+                        int32_t *starts, int32_t *slots, int64_t tokens, int32_t *counts, void *stream) {
+    if (!usable(p, gern_pipeline_s::PAGE_TABLE)) {
+        return fail("gern_page_table_run: bad pipeline");
+    }
+    if (requests < 0 || requests > GERN_PAGE_TABLE_MAX_REQUESTS) {
+        return fail("gern_page_table_run: requests must be in [0, GERN_PAGE_TABLE_MAX_REQUESTS = 8192]");
+    }
+    if (table_width < 1 || table_width > 0x7fffffff || tokens < 0 || tokens > 0x7fffffff || free_capacity < 0 || free_capacity > 0x7fffffff) {
+        return fail("gern_page_table_run: table_width must be in [1, 2^31), tokens and free_capacity in [0, 2^31)");
+    }
+    if (free_count == nullptr || starts == nullptr || counts == nullptr || (requests > 0 && (cached == nullptr || added == nullptr || table == nullptr || lengths == nullptr)) ||
+        (tokens > 0 && slots == nullptr) || (free_capacity > 0 && free_pages == nullptr)) {
+        return fail("gern_page_table_run: null buffer");
+    }
+    struct Buffer {
+        const void *at;
+        int64_t bytes;
+    };
+    const Buffer in[] = {{cached, 4 * requests}, {added, 4 * requests}, {free_pages, 4 * free_capacity}, {free_count, 4}};
+    const Buffer results[] = {{table, 4 * requests * table_width}, {lengths, 4 * requests}, {starts, 4 * (requests + 1)}, {slots, 4 * tokens}, {counts, 8}};
+    for (const auto &b : in) {
+        if (!aligned(b.at, 4)) {
+            return fail("gern_page_table_run: buffers must be 4-byte aligned");
+        }
+    }
+    for (const auto &r : results) {
+        if (!aligned(r.at, 4)) {
+            return fail("gern_page_table_run: buffers must be 4-byte aligned");
+        }
+        for (const auto &b : in) {
+            if (overlap(r.at, r.bytes, b.at, b.bytes)) {
+                return fail("gern_page_table_run: a result shares memory with an input (workgroups read the inputs while others write)");
+            }
+        }
+        for (const auto &other : results) {
+            if (&other != &r && overlap(r.at, r.bytes, other.at, other.bytes)) {
+                return fail("gern_page_table_run: two results share memory");
+            }
+        }
+    }
+    hip::RequestLengths batch{cached, added, requests};
+    hip::FreePages list{free_pages, free_count, free_capacity};
+    // a workgroup for every 1024 tokens of the slot map, at most one for each CU
+    const int64_t shares = std::clamp<int64_t>((tokens + 1023) / 1024, 1, 256);
+    hip::PageTableOut result{table, lengths, starts, slots, counts, table_width, tokens, shares};
+    return evaluate(p, requests <= 1024 ? 0 : 1, "gern_page_table_run", stream, {{"batch", &batch}, {"free_pages", &list}, {"table", &result}});
+}
+
+// --------------------------------------------------------------------------------------------- writing the cache
+
+namespace {
+
+// Checks of a cache that every operator over it makes; empty when it is fine.
+std::string cacheProblem(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, int64_t pages, int64_t heads,
+                         int64_t page_size) {
+    if (k_cache == nullptr || v_cache == nullptr || k_scales == nullptr || v_scales == nullptr) {
+        return "null cache";
+    }
+    if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 4)) {
+        return "the cache's codes must be 16-byte aligned and its scales 4-byte aligned";
+    }
+    if (heads < 1 || heads > 65535) {
+        return "heads must be in [1, 65535]";
+    }
+    if (pages < 1 || pages > 0x7fffffff / page_size) {
+        return "pages must be at least 1, and pages * page_size less than 2^31";
+    }
+    return "";
+}
+
+}  // namespace
+
+int gern_cache_write_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out) {
+    if (out == nullptr) {
+        return fail("gern_cache_write_create: null argument");
+    }
+    *out = nullptr;
+    if (!goodHeadDim(head_dim) || !goodPageSize(page_size) || !goodType(type)) {
+        return fail("gern_cache_write_create: head_dim must be 64, 128, 192 or 256, page_size 16, 32, 64 or 128, and type GERN_TYPE_BF16 or "
+                    "GERN_TYPE_F16");
+    }
+    try {
+        Draft p(gern_pipeline_s::CACHE_WRITE, flags);
+        p->head_dim = head_dim;
+        p->page_size = page_size;
+        for (int64_t threads : {64, 256}) {
+            AbstractDataTypePtr tokens(new const annot::WholeADT("tokens", "gernels::NewTokensOf<" + typeName(type) + ">"));
+            using Cache = hip::WritableCache;
+            AbstractDataTypePtr cache(new const annot::PiecesADT<Cache>("cache", "gernels::WritableCache", "at",
+                                                                       {{"stretches", &Cache::stretches}, {"heads", &Cache::heads}, {"sides", &Cache::sides}}));
+            annot::PieceFunction write("gernels::write_cache", "gernels/cache_write.h", {tokens}, cache, {"stretches", "heads", "sides"},
+                                       {"head_dim", "page", "threads"});
+            Variable x("x"), head("head"), side("side"), block("block");
+            Composable program = Global((Tile(cache["stretches"], x.bind(1)) || Grid::BLOCK_X)((Tile(cache["heads"], head.bind(1)) || Grid::BLOCK_Y)(
+                                            (Tile(cache["sides"], side.bind(1)) || Grid::BLOCK_Z)(
+                                                write[{constant("head_dim", head_dim), constant("page", page_size), constant("threads", threads)}](tokens, cache)))),
+                                        {{Grid::BLOCK_DIM_X, block.bind(threads)}});
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                return 1;
+            }
+        }
+        if (p.addFaultCount("gern_cache_write_create") != 0) {
+            return 1;
+        }
+        *out = p.handOut();
+    } catch (const std::exception &e) {
+        return fail(e.what());
+    }
+    return 0;
+}
+
+int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void *V, int64_t ldv, const int32_t *slots, int64_t tokens,
+                         int64_t heads, uint8_t *k_cache, uint8_t *v_cache, float *k_scales, float *v_scales, int64_t pages, void *stream) {
+    if (!usable(p, gern_pipeline_s::CACHE_WRITE)) {
+        return fail("gern_cache_write_run: bad pipeline");
+    }
+    const std::string problem = cacheProblem(k_cache, v_cache, k_scales, v_scales, pages, heads, p->page_size);
+    if (!problem.empty()) {
+        return fail("gern_cache_write_run: " + problem);
+    }
+    if (tokens < 0 || tokens > 0x7fffffff) {
+        return fail("gern_cache_write_run: tokens must be in [0, 2^31)");
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if (K == nullptr || V == nullptr || slots == nullptr) {
+        return fail("gern_cache_write_run: null buffer");
+    }
+    if (!aligned(K, 16) || !aligned(V, 16) || ldk % 8 != 0 || ldv % 8 != 0 || !aligned(slots, 4)) {
+        return fail("gern_cache_write_run: K and V are read in 16-byte pieces: both must be 16-byte aligned and their row strides multiples of 8 "
+                    "elements (slots 4-byte aligned)");
+    }
+    if (ldk < heads * p->head_dim || ldv < heads * p->head_dim) {
+        return fail("gern_cache_write_run: a row stride is less than heads * head_dim");
+    }
+    hip::NewTokens fresh{K, V, ldk / 2, ldv / 2, slots, tokens};
+    // One token per workgroup of one wavefront while that gives no more workgroups than the GPU runs at a time;
+    // beyond that a page's worth of tokens per workgroup of four.
+    const bool single = tokens * heads * 2 <= 16384;
+    const int64_t stretch = single ? 1 : p->page_size;
+    hip::WritableCache cache{{k_cache, v_cache, k_scales, v_scales, pages, heads, p->fault_count}, (tokens + stretch - 1) / stretch, stretch, 2};
+    return evaluate(p, single ? 0 : 1, "gern_cache_write_run", stream, {{"tokens", &fresh}, {"cache", &cache}});
+}
+
+}  // extern "C"

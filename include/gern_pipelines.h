@@ -176,6 +176,65 @@ int gern_gemm_schedule_run(gern_pipeline p, const float *A, const float *B, floa
 int gern_qk_softmax_run_no_alloc(gern_pipeline p, const uint16_t *Q, const uint16_t *K, float *S,
                                  int64_t M, int64_t N, float scale, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A serving step over a paged cache of keys and values in 8 bits.
+ *
+ * The cache: a page holds page_size (16, 32, 64 or 128) consecutive tokens of
+ * one request.  Codes are [pages, heads, page_size, head_dim] bytes in e4m3
+ * (4 exponent bits, 3 mantissa bits, +-448, no infinities), scales [pages,
+ * heads] fp32, both for keys and for values; a value is code * scale.
+ * pages * page_size is less than 2^31.  A slot is page * page_size + place.
+ * head_dim is 64, 128, 192 or 256.
+ *
+ * These pipelines keep no memory between runs (each may run on several
+ * streams, also at a time, while buffers and workspaces are not shared) and may
+ * be recorded into HIP graphs; what depends on the lengths of the requests is
+ * read on the device.  Nothing in the reference corresponds to them. */
+
+/* Types of keys, values, queries and activations. */
+enum { GERN_TYPE_BF16 = 0, GERN_TYPE_F16 = 1 };
+
+/* Block tables and slot maps, from the lengths of the requests.  Request b
+ * holds cached[b] tokens and adds added[b] (negative counts as 0).
+ *   lengths[b] = cached[b] + added[b]                     [requests]
+ *   starts[b]  = sum of added[c], c < b                   [requests + 1]
+ *   table[b, ceil(cached[b]/P) + j]                       [requests, table_width]
+ *              = the next page from the END of free_pages[0 .. *free_count),
+ *                for every page that the added tokens need, request by request
+ *   slots[t]   = the slot of added token t, t = starts[b] + i; -1 from
+ *                starts[requests] on                      [tokens]
+ *   counts     = {pages left in the free list, pages that were missing}
+ * Other entries of the table stay as they are.  A page that the free list does
+ * not have is -1 in the table, one beyond table_width is not in it; either
+ * counts as missing, and its tokens' slots are -1.  tokens may be more than is
+ * added (a captured step), or fewer.  cached, added, free_pages and *free_count
+ * are read on the device and may not share memory with the results.  The sum of
+ * cached + added is less than 2^31. */
+#define GERN_PAGE_TABLE_MAX_REQUESTS 8192
+int gern_page_table_create(int64_t page_size, int flags, gern_pipeline *out);
+int gern_page_table_run(gern_pipeline p, const int32_t *cached, const int32_t *added, int64_t requests,
+                        const int32_t *free_pages, int64_t free_capacity, const int32_t *free_count,
+                        int32_t *table, int64_t table_width, int32_t *lengths, int32_t *starts,
+                        int32_t *slots, int64_t tokens, int32_t *counts, void *stream);
+
+/* New keys and values into the cache.  K and V: [tokens, heads, head_dim] in
+ * `type`, row strides ldk and ldv in elements (multiples of 8), 16-byte aligned.
+ * Token t goes to slots[t]; a negative slot is skipped, one outside the cache
+ * is skipped and counted (gern_pipeline_faults).  The scale of a page and head
+ * is the smallest power of two (at least 2^-64) that brings what is added
+ * within +-448, or the page's old scale where that is larger and the page holds
+ * tokens in front of the added ones; codes already there move to the new scale.
+ * Values are rounded to nearest even; infinities saturate, NaN stays NaN and
+ * neither counts for the scale.
+ * Tokens of one page must be consecutive and in order in a call (as
+ * gern_page_table_run makes them): the page's tokens in front of the first one
+ * are kept, and what stands behind the last one is unspecified.  Two such runs
+ * of tokens for one page in one call race on that page. */
+int gern_cache_write_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out);
+int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void *V, int64_t ldv,
+                         const int32_t *slots, int64_t tokens, int64_t heads, uint8_t *k_cache,
+                         uint8_t *v_cache, float *k_scales, float *v_scales, int64_t pages, void *stream);
+
 /* What the kernels of the pipeline could not do and could only signal in
  * their results, since a run returns before they execute.  Waits for the
  * device, then stores in *count, and clears, the sum of
@@ -187,7 +246,8 @@ int gern_qk_softmax_run_no_alloc(gern_pipeline p, const uint16_t *Q, const uint1
  *     gern_qk_softmax_run_no_alloc count in one place per GPU, shared with
  *     the other pipelines that use it),
  *   - requests that the LDS allocator of a gern_gemm_schedule pipeline could
- *     not meet (not cleared: a count over the life of the pipeline).
+ *     not meet (not cleared: a count over the life of the pipeline),
+ *   - slots outside the cache that gern_cache_write_run skipped.
  * 0 means every result is what the pipeline computes.  Takes the place of the
  * reference's check after each launch,
  * include/gern/codegen/helpers/check_last_error.h:7-18. */

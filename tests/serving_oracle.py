@@ -1,0 +1,76 @@
+"""What the operators of a serving step compute, in 64 bits and plain loops."""
+import numpy as np
+
+E4M3_MAX = 448.0
+
+
+def e4m3_table():
+    """The value of each of the 256 codes."""
+    c = np.arange(256)
+    sign, e, m = np.where(c & 128, -1.0, 1.0), (c >> 3) & 15, c & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e.astype(np.float64) - 10))
+    v = np.where((c & 127) == 127, np.nan, v)
+    return sign * v
+
+
+def e4m3_round(x):
+    """The nearest e4m3 value, ties to even; saturates, keeps NaN."""
+    x = np.asarray(x, dtype=np.float64)
+    _, e = np.frexp(x)
+    step = np.exp2(np.maximum(np.where(np.isfinite(x), e, 0) - 4, -9).astype(np.float64))
+    with np.errstate(invalid="ignore"):
+        return np.where(np.isinf(x), np.sign(x) * E4M3_MAX, np.clip(np.rint(x / step) * step, -E4M3_MAX, E4M3_MAX))
+
+
+def scale_for(amax):
+    e = -64
+    while amax > E4M3_MAX * 2.0 ** e:
+        e += 1
+    return 2.0 ** e
+
+
+def tables(cached, added, free, count, table, page, tokens):
+    table, starts, slots, left, missing = table.copy(), [0], [], count, 0
+    cached, added = np.maximum(cached, 0), np.maximum(added, 0)
+    for b in range(len(cached)):
+        for pos in range(cached[b], cached[b] + added[b]):
+            j = pos // page
+            if pos % page == 0:
+                if j >= table.shape[1]:
+                    missing += 1
+                elif left > 0:
+                    left -= 1
+                    table[b, j] = free[left]
+                else:
+                    missing += 1
+                    table[b, j] = -1
+            held = table[b, j] if j < table.shape[1] else -1
+            slots.append(held * page + pos % page if held >= 0 else -1)
+        starts.append(len(slots))
+    slots = (slots + [-1] * tokens)[:tokens]
+    return dict(table=table, lengths=cached + added, starts=np.array(starts), slots=np.array(slots, dtype=np.int64), counts=np.array([left, missing]))
+
+
+def write(x, slots, codes, scales):
+    """codes [pages, heads, page, dim] as values; returns (codes, scales)."""
+    codes, scales, (pages, _, page, _) = codes.copy(), scales.astype(np.float64).copy(), codes.shape
+    t = 0
+    while t < len(slots):
+        n = 1
+        if slots[t] < 0 or slots[t] // page >= pages:
+            t += 1
+            continue
+        p, low = divmod(int(slots[t]), page)
+        while t + n < len(slots) and slots[t + n] == slots[t] + n and low + n < page:
+            n += 1
+        for h in range(codes.shape[1]):
+            new = x[t:t + n, h]
+            finite = np.abs(new[np.isfinite(new)])
+            need = scale_for(finite.max() if finite.size else 0.0)
+            s = max(scales[p, h], need) if low > 0 else need
+            if low > 0:
+                codes[p, h, :low] = e4m3_round(codes[p, h, :low] * (scales[p, h] / s))
+            codes[p, h, low:low + n] = e4m3_round(new / s)
+            scales[p, h] = s
+        t += n
+    return codes, scales
