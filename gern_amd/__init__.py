@@ -78,6 +78,10 @@ def _load():
     pipes.gern_page_table_run.argtypes = [vp, vp, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp]
     pipes.gern_cache_write_create.argtypes = [i64, i64, C.c_int, C.c_int, C.POINTER(vp)]
     pipes.gern_cache_write_run.argtypes = [vp, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, i64, vp]
+    pipes.gern_cache_attention_create.argtypes = [i64, i64, C.c_int, C.c_int, C.POINTER(vp)]
+    pipes.gern_cache_attention_workspace.argtypes = [vp, i64, i64, i64, i64, i64, i64, C.POINTER(i64)]
+    pipes.gern_cache_attention_run.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, vp, i64, C.c_float, i64, i64, vp,
+                                               i64, vp]
     cpp = C.POINTER(C.c_char_p)
     hip.gern_hip_compile.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(vp)]
     hip.gern_hip_compile_only.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(sz)]
@@ -411,3 +415,42 @@ class CacheWrite(_ServingPipeline):
         self._on_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
         _check(pipelines_lib().gern_cache_write_run(self.h, _ptr(k), _pitch(k), _ptr(v), _pitch(v), _ptr(slots), n, heads, _ptr(k_cache), _ptr(v_cache),
                                                     _ptr(k_scales), _ptr(v_scales), pages, stream))
+
+
+class CacheAttention(_ServingPipeline):
+    """Causal attention of ragged batches of queries over a paged cache in 8 bits (gern_cache_attention_run)."""
+
+    def __init__(self, head_dim=128, page_size=16, dtype="bf16", flags=0):
+        super().__init__()
+        self.head_dim, self.page_size, self.dtype = head_dim, page_size, dtype
+        _check(pipelines_lib().gern_cache_attention_create(head_dim, page_size, _type(dtype), flags, C.byref(self.h)))
+
+    def workspace_bytes(self, tokens, requests, q_heads, kv_heads, max_queries, max_length):
+        """Bytes of device memory that a call of these sizes needs."""
+        n = C.c_int64(-1)
+        _check(pipelines_lib().gern_cache_attention_workspace(self.h, tokens, requests, q_heads, kv_heads, max_queries, max_length, C.byref(n)))
+        return n.value
+
+    def __call__(self, q, k_cache, v_cache, k_scales, v_scales, table, lengths, starts, out, scale, max_queries=1, max_length=None, workspace=None,
+                 stream=None):
+        """q, out [tokens, q_heads, head_dim] (any stride from token to token); the cache as CacheWrite fills it; table
+        [requests, width], lengths [requests], starts [requests + 1] int32.  max_length: the most keys of a request, by
+        default what the table has room for; workspace: a uint8 tensor of workspace_bytes."""
+        pages, heads = self._cache(k_cache, v_cache, k_scales, v_scales)
+        self._int32(table=table, lengths=lengths, starts=starts)
+        self._halves(q=q, out=out)
+        n = lengths.shape[0]
+        _expect(q.dim() == 3 and q.shape[2] == self.head_dim and out.shape == q.shape, "q and out must be [tokens, q_heads, head_dim]")
+        _expect(table.dim() == 2 and table.shape[0] == n and tuple(lengths.shape) == (n,) and tuple(starts.shape) == (n + 1,),
+                "table must be [requests, width], lengths [requests] and starts [requests + 1]")
+        self._on_gpu(q, k_cache, v_cache, k_scales, v_scales, table, lengths, starts, out)
+        ws, ws_bytes = None, 0
+        if workspace is not None:
+            _expect(workspace.is_contiguous(), "the workspace must be contiguous")
+            self._on_gpu(workspace)
+            ws, ws_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
+        _check(pipelines_lib().gern_cache_attention_run(
+            self.h, _ptr(q), _pitch(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales), pages, _ptr(table), table.shape[1], _ptr(lengths),
+            _ptr(starts), n, q.shape[0], q.shape[1], heads, _ptr(out), _pitch(out), float(scale), max_queries,
+            table.shape[1] * self.page_size if max_length is None else max_length, ws, ws_bytes, stream))
+        return out

@@ -1,6 +1,6 @@
 // Annotations of the gernels over a paged 8-bit cache of keys and values
-// (gernels/paged_cache.h, page_table.h, cache_write.h), and the host mirrors
-// of their device aggregates.  Nothing in the reference corresponds to these.
+// (gernels/paged_cache.h, page_table.h, cache_write.h, cache_attention.h), and
+// the host mirrors of their device aggregates.  Nothing in the reference corresponds to these.
 #pragma once
 
 #include "annot/table.h"
@@ -39,6 +39,27 @@ struct FreePages {
 struct PageTableOut {
     int32_t *table, *lengths, *starts, *slots, *counts;
     int64_t width, tokens, shares;
+};
+
+struct AttentionBatch {
+    const void *q;
+    int64_t q_pitch;
+    const int32_t *table, *lengths, *starts;
+    int64_t width, tokens, group;
+    float scale;
+};
+struct AttentionOut {
+    void *out;
+    int64_t out_pitch;
+    float *partial, *stats;
+    int64_t splits, chunk, pieces, heads, requests;
+};
+struct JoinRows {
+    void *out;
+    int64_t out_pitch;
+    const float *partial, *stats;
+    const int32_t *starts;
+    int64_t splits, requests, q_heads, rows, blocks;
 };
 
 }  // namespace hip

@@ -153,3 +153,43 @@ __global__ void __launch_bounds__(512) check_qk_softmax_tiles(gernels::MatrixBF1
 }
 template __global__ void check_qk_softmax_tiles<128>(gernels::MatrixBF16, gernels::MatrixBF16, gernels::MatrixF32, gernels::RowStatsExchange, float);
 template __global__ void check_qk_softmax_tiles<192>(gernels::MatrixBF16, gernels::MatrixBF16, gernels::MatrixF32, gernels::RowStatsExchange, float);
+
+#include "gernels/cache_attention.h"
+#include "gernels/cache_write.h"
+#include "gernels/page_table.h"
+
+template<int64_t PER>
+__global__ void __launch_bounds__(1024) check_page_table(gernels::RequestLengths batch, gernels::FreePages free_pages, gernels::PageTableOut table) {
+    auto share = table.share(blockIdx.x);
+    gernels::extend_page_table<16, 1024, PER>(batch.whole(), free_pages.whole(), share);
+}
+template __global__ void check_page_table<1>(gernels::RequestLengths, gernels::FreePages, gernels::PageTableOut);
+template __global__ void check_page_table<8>(gernels::RequestLengths, gernels::FreePages, gernels::PageTableOut);
+
+template<int64_t D, int64_t PAGE, int64_t THREADS, class T>
+__global__ void __launch_bounds__(THREADS) check_write_cache(gernels::NewTokensOf<T> tokens, gernels::WritableCache cache) {
+    auto stretch = cache.at(blockIdx.x, blockIdx.y, blockIdx.z);
+    gernels::write_cache<D, PAGE, THREADS>(tokens.whole(), stretch);
+}
+template __global__ void check_write_cache<128, 16, 64, gernels::Bf16>(gernels::NewTokensOf<gernels::Bf16>, gernels::WritableCache);
+template __global__ void check_write_cache<64, 128, 256, gernels::F16>(gernels::NewTokensOf<gernels::F16>, gernels::WritableCache);
+
+template<int64_t D, int64_t PAGE, int64_t R, int64_t KEYS, class T>
+__global__ void __launch_bounds__(256) check_attend(gernels::AttentionBatchOf<T> batch, gernels::PagedCache cache, gernels::AttentionOut result) {
+    auto piece = result.piece(blockIdx.x, blockIdx.y, blockIdx.z);
+    gernels::attend<D, PAGE, R, 4, KEYS>(batch.whole(), cache.whole(), piece);
+}
+template __global__ void check_attend<64, 32, 1, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<64, 32, 4, 0, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<128, 64, 1, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<128, 16, 2, 0, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<192, 16, 1, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<256, 16, 1, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend<256, 16, 1, 0, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+
+template<int64_t D, class T>
+__global__ void __launch_bounds__(256) check_join_splits(gernels::AttentionBatchOf<T> batch, gernels::JoinRows rows) {
+    auto block = rows.block(blockIdx.x);
+    gernels::join_splits<D, 4>(batch.whole(), block);
+}
+template __global__ void check_join_splits<192, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::JoinRows);

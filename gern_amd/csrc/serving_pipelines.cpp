@@ -310,4 +310,183 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
     return evaluate(p, single ? 0 : 1, "gern_cache_write_run", stream, {{"tokens", &fresh}, {"cache", &cache}});
 }
 
+// --------------------------------------------------------------------------------------------- attention
+
+namespace {
+
+// How a run divides its work: which program, and the split of the keys.
+struct AttentionPlan {
+    size_t variant;
+    int64_t row_tiles, splits, chunk;
+};
+
+constexpr int64_t kMaxSplits = 64;  // gernels/cache_attention.h, join_splits
+
+// Row tiles per wavefront of the program that divides rows among wavefronts: accumulators and queries of R
+// tiles take 3/8 R D registers a lane.
+int64_t attentionRowTiles(int64_t head_dim) {
+    return head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;
+}
+
+AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, int64_t rows, int64_t max_length) {
+    AttentionPlan plan{};
+    // Up to 32 rows (queries times the heads that share a head of the cache) the wavefronts of a workgroup divide
+    // the keys, beyond that the rows.
+    plan.variant = rows <= 32 ? 0 : 1;
+    const int64_t tile = plan.variant == 0 ? 16 : 64 * attentionRowTiles(head_dim);
+    plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
+    // Keys are split until there are four workgroups for each of 256 CUs, into pieces of at least 256 keys.
+    const int64_t whole = requests * heads * plan.row_tiles;
+    const int64_t wanted = std::max<int64_t>(1, (1024 + whole - 1) / whole);
+    const int64_t chunk = std::max<int64_t>(256, (max_length + wanted - 1) / wanted);
+    plan.chunk = std::max((chunk + 127) / 128 * 128, (max_length + kMaxSplits * 128 - 1) / (kMaxSplits * 128) * 128);
+    plan.splits = std::max<int64_t>(1, (max_length + plan.chunk - 1) / plan.chunk);
+    return plan;
+}
+
+int64_t attentionWorkspace(const AttentionPlan &plan, int64_t tokens, int64_t q_heads, int64_t head_dim) {
+    return plan.splits == 1 ? 0 : plan.splits * tokens * q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+// Checks of the sizes that a run and its workspace depend on; empty when they are fine.
+std::string attentionProblem(int64_t tokens, int64_t requests, int64_t q_heads, int64_t heads, int64_t max_queries, int64_t max_length) {
+    if (heads < 1 || heads > 65535 || q_heads < heads || q_heads % heads != 0) {
+        return "heads must be in [1, 65535] and q_heads a multiple of it";
+    }
+    if (requests < 0 || requests > 65535) {
+        return "requests must be in [0, 65535]";
+    }
+    if (tokens < 0 || max_queries < 1 || max_queries > 0x7fffffff / q_heads || tokens > 0x7fffffff / q_heads) {
+        return "tokens * q_heads and max_queries * q_heads must be less than 2^31, and max_queries at least 1";
+    }
+    if (max_length < 1 || max_length > GERN_CACHE_MAX_LENGTH) {
+        return "max_length must be in [1, GERN_CACHE_MAX_LENGTH]";
+    }
+    return "";
+}
+
+}  // namespace
+
+int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out) {
+    if (out == nullptr) {
+        return fail("gern_cache_attention_create: null argument");
+    }
+    *out = nullptr;
+    if (!goodHeadDim(head_dim) || !goodPageSize(page_size) || !goodType(type)) {
+        return fail("gern_cache_attention_create: head_dim must be 64, 128, 192 or 256, page_size 16, 32, 64 or 128, and type GERN_TYPE_BF16 or "
+                    "GERN_TYPE_F16");
+    }
+    try {
+        Draft p(gern_pipeline_s::CACHE_ATTENTION, flags);
+        p->head_dim = head_dim;
+        p->page_size = page_size;
+        const std::string header = "gernels/cache_attention.h", batch_type = "gernels::AttentionBatchOf<" + typeName(type) + ">";
+        AbstractDataTypePtr batch(new const annot::WholeADT("batch", batch_type));
+        AbstractDataTypePtr cache(new const annot::WholeADT("cache", "gernels::PagedCache"));
+        for (bool keys : {true, false}) {
+            using Out = hip::AttentionOut;
+            AbstractDataTypePtr result(new const annot::PiecesADT<Out>("result", "gernels::AttentionOut", "piece",
+                                                                      {{"pieces", &Out::pieces}, {"heads", &Out::heads}, {"requests", &Out::requests}}));
+            annot::PieceFunction attend("gernels::attend", header, {batch, cache}, result, {"pieces", "heads", "requests"},
+                                        {"head_dim", "page", "row_tiles", "waves", "divide_keys"});
+            Variable x("x"), head("head"), request("request"), threads("threads");
+            Composable program = Global(
+                (Tile(result["pieces"], x.bind(1)) || Grid::BLOCK_X)((Tile(result["heads"], head.bind(1)) || Grid::BLOCK_Y)(
+                    (Tile(result["requests"], request.bind(1)) || Grid::BLOCK_Z)(
+                        attend[{constant("head_dim", head_dim), constant("page", page_size), constant("row_tiles", keys ? 1 : attentionRowTiles(head_dim)),
+                                constant("waves", 4), constant("divide_keys", keys)}](batch, cache, result)))),
+                {{Grid::BLOCK_DIM_X, threads.bind(256)}});
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                return 1;
+            }
+        }
+        using Rows = hip::JoinRows;
+        AbstractDataTypePtr rows(new const annot::PiecesADT<Rows>("rows", "gernels::JoinRows", "block", {{"blocks", &Rows::blocks}}));
+        annot::PieceFunction join("gernels::join_splits", header, {batch}, rows, {"blocks"}, {"head_dim", "waves"});
+        Variable x("x"), threads("threads");
+        Composable program = Global((Tile(rows["blocks"], x.bind(1)) || Grid::BLOCK_X)(
+                                        join[{constant("head_dim", head_dim), constant("waves", 4)}](batch, rows)),
+                                    {{Grid::BLOCK_DIM_X, threads.bind(256)}});
+        if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0 || p.addFaultCount("gern_cache_attention_create") != 0) {
+            return 1;
+        }
+        *out = p.handOut();
+    } catch (const std::exception &e) {
+        return fail(e.what());
+    }
+    return 0;
+}
+
+int gern_cache_attention_workspace(gern_pipeline p, int64_t tokens, int64_t requests, int64_t q_heads, int64_t heads, int64_t max_queries,
+                                   int64_t max_length, int64_t *bytes) {
+    if (!usable(p, gern_pipeline_s::CACHE_ATTENTION) || bytes == nullptr) {
+        return fail("gern_cache_attention_workspace: bad pipeline or null argument");
+    }
+    const std::string problem = attentionProblem(tokens, requests, q_heads, heads, max_queries, max_length);
+    if (!problem.empty()) {
+        return fail("gern_cache_attention_workspace: " + problem);
+    }
+    *bytes = requests == 0 ? 0
+                           : attentionWorkspace(attentionPlan(p->head_dim, requests, heads, max_queries * (q_heads / heads), max_length), tokens, q_heads,
+                                                p->head_dim);
+    return 0;
+}
+
+int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,
+                             const float *v_scales, int64_t pages, const int32_t *table, int64_t table_width, const int32_t *lengths,
+                             const int32_t *starts, int64_t requests, int64_t tokens, int64_t q_heads, int64_t heads, void *O, int64_t ldo,
+                             float scale, int64_t max_queries, int64_t max_length, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *who = "gern_cache_attention_run";
+    if (!usable(p, gern_pipeline_s::CACHE_ATTENTION)) {
+        return fail("gern_cache_attention_run: bad pipeline");
+    }
+    std::string problem = attentionProblem(tokens, requests, q_heads, heads, max_queries, max_length);
+    if (problem.empty()) {
+        problem = cacheProblem(k_cache, v_cache, k_scales, v_scales, pages, heads, p->page_size);
+    }
+    if (!problem.empty()) {
+        return fail("gern_cache_attention_run: " + problem);
+    }
+    if (table_width < 1 || table_width > GERN_CACHE_MAX_LENGTH / p->page_size) {
+        return fail("gern_cache_attention_run: table_width must be at least 1 and table_width * page_size at most GERN_CACHE_MAX_LENGTH");
+    }
+    if (requests == 0 || tokens == 0) {
+        return 0;
+    }
+    if (Q == nullptr || O == nullptr || table == nullptr || lengths == nullptr || starts == nullptr) {
+        return fail("gern_cache_attention_run: null buffer");
+    }
+    if (!aligned(Q, 16) || !aligned(O, 16) || ldq % 8 != 0 || ldo % 8 != 0 || !aligned(table, 4) || !aligned(lengths, 4) || !aligned(starts, 4)) {
+        return fail("gern_cache_attention_run: Q and O are moved in 16-byte pieces: both must be 16-byte aligned and their row strides multiples of 8 "
+                    "elements (table, lengths and starts 4-byte aligned)");
+    }
+    if (ldq < q_heads * p->head_dim || ldo < q_heads * p->head_dim) {
+        return fail("gern_cache_attention_run: a row stride is less than q_heads * head_dim");
+    }
+    const int64_t group = q_heads / heads;
+    const AttentionPlan plan = attentionPlan(p->head_dim, requests, heads, max_queries * group, max_length);
+    const int64_t needed = attentionWorkspace(plan, tokens, q_heads, p->head_dim);
+    if (needed > 0 && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 16))) {
+        return fail("gern_cache_attention_run: the workspace must be 16-byte aligned and hold the " + std::to_string(needed) +
+                    " bytes that gern_cache_attention_workspace says");
+    }
+    if (needed > 0 && overlap(workspace, needed, O, ((tokens - 1) * ldo + q_heads * p->head_dim) * 2)) {
+        return fail("gern_cache_attention_run: the workspace shares memory with O");
+    }
+    const int64_t rows = tokens * q_heads;
+    float *partial = static_cast<float *>(workspace), *stats = needed > 0 ? partial + plan.splits * rows * p->head_dim : nullptr;
+    hip::AttentionBatch batch{Q, ldq / 2, table, lengths, starts, table_width, tokens, group, scale * 1.4426950408889634f};
+    hip::PagedCache cache{const_cast<uint8_t *>(k_cache), const_cast<uint8_t *>(v_cache), const_cast<float *>(k_scales), const_cast<float *>(v_scales),
+                          pages, heads, p->fault_count};
+    hip::AttentionOut result{O, ldo / 2, partial, stats, plan.splits, plan.chunk, plan.row_tiles * plan.splits, heads, requests};
+    const int rc = evaluate(p, plan.variant, who, stream, {{"batch", &batch}, {"cache", &cache}, {"result", &result}});
+    if (rc != 0 || plan.splits == 1) {
+        return rc;
+    }
+    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, (rows + 3) / 4};
+    const int joined = evaluate(p, 2, who, stream, {{"batch", &batch}, {"rows", &join}});
+    p->last_variant = plan.variant;
+    return joined;
+}
+
 }  // extern "C"

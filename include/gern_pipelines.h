@@ -235,6 +235,37 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
                          const int32_t *slots, int64_t tokens, int64_t heads, uint8_t *k_cache,
                          uint8_t *v_cache, float *k_scales, float *v_scales, int64_t pages, void *stream);
 
+/* Attention over the cache.  Request r's queries are rows starts[r] ..
+ * starts[r + 1] of Q (a token each, [tokens, q_heads, head_dim] in `type`, row
+ * stride ldq), its keys the lengths[r] tokens that row r of table names; the
+ * queries are the last of them: query i of n sees the keys up to
+ * lengths[r] - n + i.  q_heads / heads consecutive heads of Q share a head of
+ * the cache.
+ *   O = softmax(scale * q . k) v over the keys a query sees, 0 where it sees none
+ * (a request of length 0, a query in front of the first key), in `type`, row
+ * stride ldo; rows of Q in no request are left alone in O.
+ * max_queries and max_length tell the most queries and keys of one request; the
+ * division of the work and the workspace depend on them and the results do not
+ * (more are computed, too, only slower).  The workspace
+ * (gern_cache_attention_workspace bytes, 16-byte aligned, any content) is the
+ * call's from its launch to its end: calls that overlap in time need one each.
+ * One launch, or two where the keys are split among workgroups.
+ * Keys on a page that is not in the cache (a table entry outside [0, pages), or
+ * lengths[r] beyond the table) are left out, and gern_pipeline_faults is not 0
+ * then.  What stands behind the last key, in its page or in the table, is not
+ * used, whatever it is. */
+#define GERN_CACHE_MAX_LENGTH (1 << 30)
+int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out);
+int gern_cache_attention_workspace(gern_pipeline p, int64_t tokens, int64_t requests, int64_t q_heads,
+                                   int64_t heads, int64_t max_queries, int64_t max_length, int64_t *bytes);
+int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const uint8_t *k_cache,
+                             const uint8_t *v_cache, const float *k_scales, const float *v_scales,
+                             int64_t pages, const int32_t *table, int64_t table_width,
+                             const int32_t *lengths, const int32_t *starts, int64_t requests,
+                             int64_t tokens, int64_t q_heads, int64_t heads, void *O, int64_t ldo,
+                             float scale, int64_t max_queries, int64_t max_length, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
 /* What the kernels of the pipeline could not do and could only signal in
  * their results, since a run returns before they execute.  Waits for the
  * device, then stores in *count, and clears, the sum of
@@ -247,7 +278,9 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  *     the other pipelines that use it),
  *   - requests that the LDS allocator of a gern_gemm_schedule pipeline could
  *     not meet (not cleared: a count over the life of the pipeline),
- *   - slots outside the cache that gern_cache_write_run skipped.
+ *   - runs of slots outside the cache that gern_cache_write_run skipped,
+ *   - wavefronts of gern_cache_attention_run that met a page outside the cache,
+ *     and requests longer than the table.
  * 0 means every result is what the pipeline computes.  Takes the place of the
  * reference's check after each launch,
  * include/gern/codegen/helpers/check_last_error.h:7-18. */

@@ -74,3 +74,27 @@ def write(x, slots, codes, scales):
             scales[p, h] = s
         t += n
     return codes, scales
+
+
+def attention(q, k, v, v_scales, limits, scale):
+    """One head of one request: q [n, dim], k and v [length, dim], v_scales [length], limits[i] keys seen by query i.
+    Returns the result and how far a kernel may be from it before it rounds its result, from
+      the weights' rounding to fp16: 2^-11 of a weight, or 2^-25 of the largest one where that is more (fp16 has 11 bits
+        down to 2^-14 and steps of 2^-24 below; the largest weight, with its value scale, stands for 1)
+      the exponents: dim products summed in fp32 in steps of 32 of a matrix instruction, times a scale, plus the value
+        scale's logarithm (up to 64); once in the weights and once in their sum
+      the sums over the keys in fp32, 32 at a time, joined at the end."""
+    n, dim = q.shape
+    o, tol = np.zeros((n, dim)), np.zeros((n, dim))
+    codes = np.abs(v) / np.where(v_scales > 0, v_scales, 1.0)[:, None]
+    for i in range(n):
+        m = int(limits[i])
+        if m <= 0:
+            continue
+        z = (k[:m] @ q[i]) * scale
+        exponent = ((dim / 32 + 8) * 2.0 ** -24 * (np.abs(k[:m]) @ np.abs(q[i])) * scale + 8 * 2.0 ** -24 * (np.abs(z) + 64)).max()
+        p = np.exp(z - z.max())
+        p /= p.sum()
+        o[i] = p @ v[:m]
+        tol[i] = (2.0 ** -11 + 2 * exponent + (m / 32 + 16) * 2.0 ** -24) * (p @ np.abs(v[:m])) + 2.0 ** -25 * codes[:m].sum(axis=0) * (p * v_scales[:m]).max()
+    return o, tol

@@ -215,3 +215,264 @@ def test_write_nothing(torch, gpu):
     (kc, ks, *_), (vc, vs, *_) = [fresh_cache(torch, rs, 1, 1, 16, 64) for _ in range(2)]
     none = torch.zeros((0, 1, 64), dtype=torch.bfloat16, device="cuda")
     w(none, none, i32(torch, []), kc, vc, ks, vs)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+HALF_STEP = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}  # torch.finfo(t).eps / 2, relative to the value
+
+
+def attention_inputs(torch, dtype, dim, page, heads, group, lengths, queries, seed, value_exponents=(-4, 4), q_sigma=1.0):
+    """Tensors of a batch over a cache whose unused pages, tails and table entries hold anything."""
+    rs = np.random.RandomState(seed)
+    t = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    lengths, queries = np.array(lengths), np.array(queries)
+    held = -(-lengths // page)
+    pages = int(held.sum()) + 3
+    order = rs.permutation(pages)
+    width = int(held.max()) + 2
+    table = rs.choice([-1, 2 ** 31 - 1, -2 ** 31, pages], size=(len(lengths), width)).astype(np.int64)
+    codes = rs.randint(0, 256, (2, pages, heads, page, dim)).astype(np.uint8)
+    codes[(codes & 127) == 127] = 8
+    scales = np.stack([np.exp2(rs.randint(-9, -6, (pages, heads))), np.exp2(rs.randint(*value_exponents, (pages, heads)))]) * rs.choice([1.0, 1.37], (2, pages, heads))
+    used = np.zeros((pages, page), dtype=bool)
+    at = 0
+    for b, n in enumerate(lengths):
+        mine = order[at:at + held[b]]
+        table[b, :held[b]] = mine
+        at += held[b]
+        for i, p in enumerate(mine):
+            used[p, :max(0, min(page, n - i * page))] = True
+    codes[:, ~used.any(axis=1)] = 127
+    scales[:, ~used.any(axis=1)] = rs.choice([np.nan, np.inf], 1)
+    for p in np.flatnonzero(used.any(axis=1)):
+        codes[:, p][:, :, ~used[p]] = rs.choice([127, 255], 1)
+    scales = scales.astype(np.float32)
+    starts = np.concatenate([[0], np.cumsum(queries)])
+    tokens = int(starts[-1]) + 3  # rows behind the last request
+    rows = torch.from_numpy(rs.normal(size=(tokens, heads * group + 2, dim)) * q_sigma).to(t)
+    out = torch.full((tokens, heads * group + 1, dim), 77.0, dtype=t, device="cuda")
+    device = dict(q=rows.cuda()[:, :heads * group], k_cache=torch.from_numpy(codes[0]).cuda(), v_cache=torch.from_numpy(codes[1]).cuda(),
+                  k_scales=torch.from_numpy(scales[0]).cuda(), v_scales=torch.from_numpy(scales[1]).cuda(), table=i32(torch, table), lengths=i32(torch, lengths),
+                  starts=i32(torch, starts), out=out[:, :heads * group])
+    host = dict(q=rows[:, :heads * group].double().numpy(), codes=E4M3[codes], scales=scales.astype(np.float64), table=table, lengths=lengths, starts=starts)
+    return device, host, out
+
+
+def check_attention(out, host, dtype, page, group, scale):
+    o = out.double().cpu().numpy()
+    tokens, starts = o.shape[0], host["starts"]
+    heads, dim = host["codes"].shape[2], host["codes"].shape[4]
+    assert np.array_equal(o[starts[-1]:], np.full(o[starts[-1]:].shape, 77.0)) and np.all(o[:, heads * group:] == 77.0)
+    worst = 0.0
+    for b, n in enumerate(host["lengths"]):
+        m = starts[b + 1] - starts[b]
+        pages = host["table"][b, :-(-n // page)]
+        for h in range(heads):
+            with np.errstate(invalid="ignore"):
+                k, v = ((host["codes"][s][pages, h] * host["scales"][s][pages, h][:, None, None]).reshape(-1, dim)[:n] for s in (0, 1))
+                vs = np.repeat(host["scales"][1][pages, h], page)[:n]
+            for u in range(h * group, (h + 1) * group):
+                q, got = host["q"][starts[b]:starts[b + 1], u], o[starts[b]:starts[b + 1], u]
+                want, tol = so.attention(q, k, v, vs, n - m + np.arange(m) + 1, scale)
+                tol = tol + HALF_STEP[dtype] * (np.abs(want) + tol) + 2.0 ** -25  # the result's rounding, and fp16's smallest step
+                err = np.abs(got - want)
+                assert np.all(np.isfinite(got)), (b, u)
+                worst = max(worst, float((err / tol).max()) if m else 0.0)
+                assert np.all(err <= tol), (b, u, worst)
+    return worst
+
+
+def run_attention(torch, gpu, dtype, dim, page, heads, group, lengths, queries, seed=0, scale=None, max_queries=None, max_length=None, faults=0, **kw):
+    device, host, out = attention_inputs(torch, dtype, dim, page, heads, group, lengths, queries, seed, **kw)
+    scale = scale or 1.0 / np.sqrt(dim)
+    a = gpu("CacheAttention", head_dim=dim, page_size=page, dtype=dtype)
+    max_queries, max_length = max_queries or max(1, max(queries)), max_length or max(1, max(lengths))
+    n = a.workspace_bytes(device["q"].shape[0], len(lengths), heads * group, heads, max_queries, max_length)
+    ws = torch.full((n + 64,), 255, dtype=torch.uint8, device="cuda")
+    a(**device, scale=scale, max_queries=max_queries, max_length=max_length, workspace=ws)
+    torch.cuda.synchronize()
+    assert a.faults() == faults
+    assert torch.all(ws[n:] == 255)
+    check_attention(out, host, dtype, page, group, scale)
+    return out, n
+
+
+LENGTHS = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 300]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim, page", [(64, 16), (64, 64), (128, 16), (128, 32), (128, 128), (192, 32), (256, 16), (256, 128)])
+def test_attention_single_queries(torch, gpu, dtype, dim, page):
+    run_attention(torch, gpu, dtype, dim, page, 2, 4, LENGTHS, [1] * len(LENGTHS), seed=dim + page)
+
+
+@pytest.mark.parametrize("heads, group", [(1, 1), (3, 1), (1, 16), (2, 3), (1, 17), (1, 40), (5, 7)])
+def test_attention_head_layouts(torch, gpu, heads, group):
+    run_attention(torch, gpu, "bf16", 128, 16, heads, group, [1, 40, 129, 513], [1, 1, 1, 1], seed=heads)
+
+
+@pytest.mark.parametrize("dim, page, group", [(64, 16, 4), (128, 32, 2), (192, 16, 1), (256, 64, 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_several_queries(torch, gpu, dtype, dim, page, group):
+    """Drafted tokens (few rows) and pieces of prompts (many); requests without queries, without keys, with more queries than keys."""
+    run_attention(torch, gpu, dtype, dim, page, 2, group, [70, 5, 33, 0, 128], [3, 5, 2, 1, 4], seed=1)
+    run_attention(torch, gpu, dtype, dim, page, 2, group, [0, 0, 9, 300, 150, 200, 64], [0, 2, 20, 130, 150, 1, 0], seed=2)
+
+
+def test_attention_rows_that_see_nothing(torch, gpu):
+    for queries in (1, 100):
+        device, host, out = attention_inputs(torch, "bf16", 128, 16, 1, 4, [0, 1], [queries, queries], seed=4)
+        a = gpu("CacheAttention", head_dim=128, page_size=16, dtype="bf16")
+        a(**device, scale=0.1, max_queries=queries, max_length=64)
+        torch.cuda.synchronize()
+        assert torch.all(out[:2 * queries - 1, :4] == 0)  # nothing, or queries in front of the first key
+        check_attention(out, host, "bf16", 16, 4, 0.1)
+
+
+@pytest.mark.parametrize("dtype, dim, page, heads, group, length, queries", [
+    ("bf16", 128, 16, 1, 4, 5000, 1), ("f16", 64, 128, 2, 1, 9001, 2), ("f16", 256, 64, 1, 8, 4097, 3), ("bf16", 192, 32, 1, 2, 3001, 40), ("bf16", 64, 16, 1, 1, 70001, 1)])
+def test_attention_split_keys(torch, gpu, dtype, dim, page, heads, group, length, queries):
+    """Few long contexts: the keys are divided among workgroups and joined; a short request and an empty one beside them."""
+    _, bytes_split = run_attention(torch, gpu, dtype, dim, page, heads, group, [length, 100, 0], [queries, 1, 1], seed=length)
+    assert bytes_split > 0
+
+
+def test_attention_division_does_not_matter(torch, gpu):
+    """max_queries and max_length choose the division of the work; every choice is within the tolerance, and a run repeats itself to the bit."""
+    for max_length in (1, 300, 1000, 5000, 1 << 20):
+        for max_queries in (1, 2, 7, 500):
+            out, _ = run_attention(torch, gpu, "bf16", 128, 16, 2, 3, [1000, 37], [7, 2], seed=5, max_queries=max_queries, max_length=max_length)
+            again, _ = run_attention(torch, gpu, "bf16", 128, 16, 2, 3, [1000, 37], [7, 2], seed=5, max_queries=max_queries, max_length=max_length)
+            assert torch.equal(out, again)
+
+
+def test_attention_scales_far_apart(torch, gpu):
+    """Pages of values whose scales differ by 2^60 beside one another, and sharp and flat distributions."""
+    for sigma in (0.0, 0.1, 30.0):
+        run_attention(torch, gpu, "bf16", 128, 16, 2, 2, [400, 33], [1, 3], seed=6, value_exponents=(-50, 10), q_sigma=sigma)
+
+
+def test_attention_values_without_scale(torch, gpu):
+    """A page whose scale of values is 0 weighs in the softmax and adds nothing."""
+    device, host, out = attention_inputs(torch, "f16", 64, 16, 1, 2, [50, 16], [1, 1], seed=7)
+    for b, p in ((0, 1), (1, 0)):
+        page = host["table"][b, p]
+        device["v_scales"][page] = 0.0
+        host["scales"][1][page] = 0.0
+    a = gpu("CacheAttention", head_dim=64, page_size=16, dtype="f16")
+    a(**device, scale=0.125, max_queries=1, max_length=50)
+    torch.cuda.synchronize()
+    check_attention(out, host, "f16", 16, 2, 0.125)
+
+
+@pytest.mark.parametrize("queries", [1, 50])
+def test_attention_leaves_out_pages_outside_the_cache(torch, gpu, queries):
+    dim, page = 128, 16
+    device, host, out = attention_inputs(torch, "bf16", dim, page, 1, 2, [90, 64], [queries, 1], seed=8)
+    for bad in (-1, device["k_cache"].shape[0], 2 ** 31 - 1):
+        device["table"][0, 2] = bad
+        a = gpu("CacheAttention", head_dim=dim, page_size=page, dtype="bf16")
+        a(**device, scale=0.09, max_queries=queries, max_length=90)
+        torch.cuda.synchronize()
+        assert a.faults() > 0 and a.faults() == 0
+        o = out.double().cpu().numpy()
+        pages = host["table"][0, :6]
+        k, v = ((host["codes"][s][pages, 0] * host["scales"][s][pages, 0][:, None, None]).reshape(-1, dim)[:90] for s in (0, 1))
+        vs = np.repeat(host["scales"][1][pages, 0], page)[:90]
+        kept = np.r_[0:32, 48:90]
+        for i in range(queries):
+            seen = kept[kept < 90 - queries + i + 1]
+            for u in range(2):
+                want, tol = so.attention(host["q"][i:i + 1, u], k[seen], v[seen], vs[seen], [len(seen)], 0.09)
+                assert np.all(np.abs(o[i, u] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol))
+
+
+def test_attention_length_beyond_the_table(torch, gpu):
+    device, host, out = attention_inputs(torch, "bf16", 64, 16, 1, 1, [64, 20], [1, 1], seed=9)
+    device["table"] = device["table"][:, :4].contiguous()
+    device["lengths"][0] = 1000
+    a = gpu("CacheAttention", head_dim=64, page_size=16, dtype="bf16")
+    a(**device, scale=0.125, max_queries=1, max_length=64)
+    torch.cuda.synchronize()
+    assert a.faults() == 1
+    check_attention(out, host, "bf16", 16, 1, 0.125)
+
+
+# ------------------------------------------------------------------------------------------------ a step
+
+
+def test_a_serving_step(torch, gpu):
+    """Tables, write and attention as a server calls them: prompts, then tokens one at a time, replayed from a graph."""
+    dim, page, heads, group, requests, pages = 128, 16, 2, 4, 3, 40
+    rs = np.random.RandomState(12)
+    tables, write, attend = (gpu(n, **k) for n, k in (("PageTable", dict(page_size=page)), ("CacheWrite", dict(head_dim=dim, page_size=page, dtype="bf16")),
+                                                      ("CacheAttention", dict(head_dim=dim, page_size=page, dtype="bf16"))))
+    width, most = 12, 60
+    state = dict(cached=i32(torch, [0] * requests), added=i32(torch, [0] * requests), free=i32(torch, rs.permutation(pages)), count=i32(torch, [pages]),
+                 table=i32(torch, np.full((requests, width), -1)), lengths=i32(torch, [0] * requests), starts=i32(torch, [0] * (requests + 1)),
+                 slots=i32(torch, [0] * most), counts=i32(torch, [0, 0]))
+    kc, vc = (torch.full((pages, heads, page, dim), 127, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((pages, heads), float("nan"), device="cuda") for _ in range(2))
+    qkv = torch.zeros((most, heads * (group + 2), dim), dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros((most, heads * group, dim), dtype=torch.bfloat16, device="cuda")
+    ws = torch.zeros(attend.workspace_bytes(most, requests, heads * group, heads, most, width * page), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(stream):
+        q, k, v = qkv[:, :heads * group], qkv[:, heads * group:heads * (group + 1)], qkv[:, heads * (group + 1):]
+        tables(state["cached"], state["added"], state["free"], state["count"], state["table"], state["lengths"], state["starts"], state["slots"],
+               state["counts"], stream=stream)
+        write(k, v, state["slots"], kc, vc, ks, vs, stream=stream)
+        attend(q, kc, vc, ks, vs, state["table"], state["lengths"], state["starts"], out, dim ** -0.5, max_queries=most, max_length=width * page, workspace=ws,
+               stream=stream)
+
+    with torch.cuda.stream(side):
+        step(side.cuda_stream)  # adds nothing: no request has tokens yet
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(side.cuda_stream)
+
+    keys = [[np.zeros((0, heads, dim))] * 2 for _ in range(requests)]  # of each request, before they are coded
+    for turn, added in enumerate([[20, 1, 33], [1, 1, 1], [1, 0, 1], [1, 16, 1], [14, 1, 0], [1, 1, 1]]):
+        state["added"].copy_(i32(torch, added))
+        fresh = rs.normal(size=tuple(qkv.shape))
+        qkv.copy_(torch.from_numpy(fresh).bfloat16())
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+        if turn % 2 == 0:
+            graph.replay()
+        else:
+            step(None)
+        torch.cuda.synchronize()
+        assert int(state["counts"][1]) == 0 and write.faults() == 0 and attend.faults() == 0
+        starts = np.concatenate([[0], np.cumsum(added)])
+        assert np.array_equal(state["starts"].cpu().numpy(), starts)
+        x = qkv.double().cpu().numpy()
+        got = out.double().cpu().numpy()
+        assert np.all(got[starts[-1]:] == 5.0)
+        scales = [ks.cpu().numpy().astype(np.float64), vs.cpu().numpy().astype(np.float64)]
+        table = state["table"].cpu().numpy()
+        for b in range(requests):
+            mine = x[starts[b]:starts[b + 1]]
+            for side_of in (0, 1):
+                at = heads * (group + side_of)
+                keys[b][side_of] = np.concatenate([keys[b][side_of], mine[:, at:at + heads]])
+            n = len(keys[b][0])
+            held = table[b, :-(-n // page)]
+            for h in range(heads):
+                coded = []
+                for side_of, codes in ((0, kc), (1, vc)):
+                    value = (E4M3[codes.cpu().numpy()[held, h]] * scales[side_of][held, h][:, None, None]).reshape(-1, dim)[:n]
+                    # a code is half a step from its value (2^-4 of it, or 2^-10 of the scale), once more for every time the
+                    # page's scale doubled, which loses under the smallest step only
+                    bound = np.abs(keys[b][side_of][:, h]) * 2.0 ** -4 + np.repeat(scales[side_of][held, h], page)[:n, None] * 2.0 ** -10 * 3
+                    assert np.all(np.abs(value - keys[b][side_of][:, h]) <= bound)
+                    coded.append(value)
+                for u in range(h * group, (h + 1) * group):
+                    want, tol = so.attention(mine[:, u], coded[0], coded[1], np.repeat(scales[1][held, h], page)[:n], n - len(mine) + np.arange(len(mine)) + 1,
+                                             dim ** -0.5)
+                    assert np.all(np.abs(got[starts[b]:starts[b + 1], u] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol)), (turn, b, u)
+        state["cached"].copy_(state["lengths"])
+        state["count"].copy_(state["counts"][:1])
