@@ -82,6 +82,8 @@ def _load():
     pipes.gern_cache_attention_workspace.argtypes = [vp, i64, i64, i64, i64, i64, i64, C.POINTER(i64)]
     pipes.gern_cache_attention_run.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, vp, i64, C.c_float, i64, i64, vp,
                                                i64, vp]
+    pipes.gern_matvec4_create.argtypes = [i64, C.c_int, C.c_int, C.POINTER(vp)]
+    pipes.gern_matvec4_run.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, i64, i64, i64, vp]
     cpp = C.POINTER(C.c_char_p)
     hip.gern_hip_compile.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(vp)]
     hip.gern_hip_compile_only.argtypes = [C.c_char_p, cpp, C.c_int, cpp, C.c_int, C.c_char_p, C.POINTER(sz)]
@@ -454,3 +456,29 @@ class CacheAttention(_ServingPipeline):
             _ptr(starts), n, q.shape[0], q.shape[1], heads, _ptr(out), _pitch(out), float(scale), max_queries,
             table.shape[1] * self.page_size if max_length is None else max_length, ws, ws_bytes, stream))
         return out
+
+
+class Matvec4(_ServingPipeline):
+    """y = x W^T for up to 64 rows of x and W in 4 bits with scales (and zero points) of groups of columns (gern_matvec4_run)."""
+
+    def __init__(self, group=128, dtype="bf16", flags=0):
+        super().__init__()
+        self.group, self.dtype = group, dtype
+        _check(pipelines_lib().gern_matvec4_create(group, _type(dtype), flags, C.byref(self.h)))
+
+    def __call__(self, x, codes, scales, y, zeros=None, stream=None):
+        """x [rows, K] and y [rows, N] (any stride from row to row); codes [N, K / 2] uint8, the even column in the lower
+        half; scales [K / group, N] of x's type; zeros [K / group, N] uint8, by default 8 everywhere."""
+        uint8 = self._torch.uint8
+        self._halves(x=x, scales=scales, y=y)
+        _expect(x.dim() == y.dim() == codes.dim() == scales.dim() == 2 and y.shape[0] == x.shape[0], "x must be [rows, K], y [rows, N], codes [N, K / 2]")
+        (m, k), n = x.shape, y.shape[1]
+        _expect(codes.dtype is uint8 and codes.is_contiguous() and codes.shape == (n, k // 2), "codes must be a contiguous uint8 tensor [N, K / 2]")
+        _expect(scales.is_contiguous() and scales.shape == (k // self.group, n), "scales must be contiguous, [K / group, N]")
+        self._on_gpu(x, codes, scales, y)
+        if zeros is not None:
+            _expect(zeros.dtype is uint8 and zeros.is_contiguous() and zeros.shape == scales.shape, "zeros must be a contiguous uint8 tensor [K / group, N]")
+            self._on_gpu(zeros)
+        _check(pipelines_lib().gern_matvec4_run(self.h, _ptr(x), _pitch(x), _ptr(codes), _ptr(scales), None if zeros is None else _ptr(zeros), _ptr(y),
+                                                _pitch(y), m, n, k, stream))
+        return y

@@ -193,3 +193,15 @@ __global__ void __launch_bounds__(256) check_join_splits(gernels::AttentionBatch
     gernels::join_splits<D, 4>(batch.whole(), block);
 }
 template __global__ void check_join_splits<192, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::JoinRows);
+
+#include "gernels/matvec4.h"
+
+template<int64_t G, int64_t MT, int64_t NT, class T>
+__global__ void __launch_bounds__(512) check_matvec4(gernels::ActivationsOf<T> x, gernels::Weights4 weights, gernels::MatvecOut y) {
+    auto columns = y.at(blockIdx.x);
+    gernels::multiply_4bit<G, MT, NT, 8>(x.whole(), weights.whole(), columns);
+}
+template __global__ void check_matvec4<128, 1, 1, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<128, 1, 2, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<64, 2, 2, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<32, 4, 2, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);

@@ -5,6 +5,7 @@
 // the grid.
 #include "pipeline.h"
 
+#include "annot/matvec4.h"
 #include "annot/paged_cache.h"
 #include "gern_hip.h"
 
@@ -487,6 +488,89 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     const int joined = evaluate(p, 2, who, stream, {{"batch", &batch}, {"rows", &join}});
     p->last_variant = plan.variant;
     return joined;
+}
+
+// --------------------------------------------------------------------------------------------- 4-bit weights
+
+namespace {
+
+struct MatvecShape {
+    int64_t row_tiles, column_tiles;
+};
+// The programs of a pipeline; 8 wavefronts each.
+constexpr MatvecShape kMatvecShapes[] = {{1, 1}, {1, 2}, {2, 2}, {4, 2}};
+constexpr int64_t kMatvecWaves = 8;
+
+}  // namespace
+
+int gern_matvec4_create(int64_t group, int type, int flags, gern_pipeline *out) {
+    if (out == nullptr) {
+        return fail("gern_matvec4_create: null argument");
+    }
+    *out = nullptr;
+    if ((group != 32 && group != 64 && group != 128) || !goodType(type)) {
+        return fail("gern_matvec4_create: group must be 32, 64 or 128, and type GERN_TYPE_BF16 or GERN_TYPE_F16");
+    }
+    try {
+        Draft p(gern_pipeline_s::MATVEC4, flags);
+        p->group = group;
+        for (const MatvecShape &shape : kMatvecShapes) {
+            AbstractDataTypePtr x(new const annot::WholeADT("x", "gernels::ActivationsOf<" + typeName(type) + ">"));
+            AbstractDataTypePtr weights(new const annot::WholeADT("weights", "gernels::Weights4"));
+            AbstractDataTypePtr y(new const annot::PiecesADT<hip::MatvecOut>("y", "gernels::MatvecOut", "at", {{"columns", &hip::MatvecOut::columns}}));
+            annot::PieceFunction multiply("gernels::multiply_4bit", "gernels/matvec4.h", {x, weights}, y, {"columns"},
+                                          {"group", "row_tiles", "column_tiles", "waves"});
+            Variable column("column"), threads("threads");
+            Composable program =
+                Global((Tile(y["columns"], column.bind(1)) || Grid::BLOCK_X)(
+                           multiply[{constant("group", group), constant("row_tiles", shape.row_tiles), constant("column_tiles", shape.column_tiles),
+                                     constant("waves", kMatvecWaves)}](x, weights, y)),
+                       {{Grid::BLOCK_DIM_X, threads.bind(64 * kMatvecWaves)}});
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                return 1;
+            }
+        }
+        *out = p.handOut();
+    } catch (const std::exception &e) {
+        return fail(e.what());
+    }
+    return 0;
+}
+
+int gern_matvec4_run(gern_pipeline p, const void *X, int64_t ldx, const uint8_t *codes, const void *scales, const uint8_t *zeros, void *Y, int64_t ldy,
+                     int64_t M, int64_t N, int64_t K, void *stream) {
+    if (!usable(p, gern_pipeline_s::MATVEC4)) {
+        return fail("gern_matvec4_run: bad pipeline");
+    }
+    if (M < 0 || M > GERN_MATVEC4_MAX_ROWS || N < 1 || N > 0x7fffffff || K < 1 || K > 0x7fffffff || K % p->group != 0) {
+        return fail("gern_matvec4_run: M must be in [0, GERN_MATVEC4_MAX_ROWS = 64], N and K in [1, 2^31), and K a multiple of the group");
+    }
+    if (M == 0) {
+        return 0;
+    }
+    if (X == nullptr || codes == nullptr || scales == nullptr || Y == nullptr) {
+        return fail("gern_matvec4_run: null buffer");
+    }
+    if (!aligned(X, 16) || ldx % 8 != 0 || !aligned(codes, 16) || !aligned(scales, 2) || !aligned(Y, 2)) {
+        return fail("gern_matvec4_run: X and the codes are read in 16-byte pieces: both must be 16-byte aligned and the row stride of X a multiple of 8 "
+                    "elements (scales and Y 2-byte aligned)");
+    }
+    if (M > 1 && (ldx < K || ldy < N)) {
+        return fail("gern_matvec4_run: a row stride is less than its row");
+    }
+    const int64_t x_bytes = ((M - 1) * ldx + K) * 2, y_bytes = ((M - 1) * ldy + N) * 2, groups = K / p->group;
+    if (overlap(Y, y_bytes, X, x_bytes) || overlap(Y, y_bytes, codes, N * K / 2) || overlap(Y, y_bytes, scales, groups * N * 2) ||
+        overlap(Y, y_bytes, zeros, zeros != nullptr ? groups * N : 0)) {
+        return fail("gern_matvec4_run: Y shares memory with an input");
+    }
+    // Two tiles of 16 columns a workgroup, so that x is read for 32 columns at a time; one where that leaves fewer
+    // workgroups than two for each of 256 CUs.
+    const size_t variant = M > 32 ? 3 : M > 16 ? 2 : N > 16384 ? 1 : 0;
+    const int64_t tile = 16 * kMatvecShapes[variant].column_tiles;
+    hip::Activations x{X, ldx / 2, M};
+    hip::Weights4 weights{codes, scales, zeros, N, K};
+    hip::MatvecOut y{Y, ldy, (N + tile - 1) / tile};
+    return evaluate(p, variant, "gern_matvec4_run", stream, {{"x", &x}, {"weights", &weights}, {"y", &y}});
 }
 
 }  // extern "C"

@@ -37,6 +37,7 @@
 // are loaded one 32-key step ahead, page numbers two.
 #pragma once
 
+#include "gernels/half_tiles.h"
 #include "gernels/paged_cache.h"
 
 namespace gernels {
@@ -82,25 +83,6 @@ __device__ __forceinline__ AttentionPiece AttentionOut::piece(int64_t x, int64_t
 
 namespace detail {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-struct Frag {
-    uint32_t w[4];
-};
-
-// C += A B on 16 x 16 x 32: lane (g, c) holds row / column c of A / B at k = 8g .. 8g+7,
-// and rows 4g .. 4g+3 of column c of C.
-template<bool BF16>
-__device__ __forceinline__ f32x4 mfma_16x16x32(const Frag &a, const Frag &b, f32x4 c) {
-    if constexpr (BF16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    }
-}
-
 // Two e4m3 codes (the low or the high two of a word) as bf16 or fp16; exact.
 template<bool BF16, bool HIGH>
 __device__ __forceinline__ uint32_t codes_to_halves(uint32_t w) {
@@ -124,23 +106,6 @@ __device__ __forceinline__ float max_over_lane_groups(float x) {
 }
 __device__ __forceinline__ float sum_over_lane_groups(float x) {
     return over_lane_groups(x, [](float a, float b) { return a + b; });
-}
-
-// N words from memory in as few loads as their alignment allows (N D-dependent: 1 .. 4).
-template<int N>
-__device__ __forceinline__ void load_words(uint32_t *to, const uint32_t *from) {
-    if constexpr (N == 4) {
-        const Words4 x = *reinterpret_cast<const Words4 *>(from);
-        to[0] = x.w[0], to[1] = x.w[1], to[2] = x.w[2], to[3] = x.w[3];
-    } else if constexpr (N == 2) {
-        const Words2 x = *reinterpret_cast<const Words2 *>(from);
-        to[0] = x.w[0], to[1] = x.w[1];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            to[i] = from[i];
-        }
-    }
 }
 
 // Below every score; finite, so that a row that has seen nothing yet gives 2^(-inf - m) = 0.

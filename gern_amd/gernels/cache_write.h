@@ -20,6 +20,7 @@
 // in consecutive slots of one page.  A run is the first token's workgroup's.
 #pragma once
 
+#include "gernels/half_tiles.h"
 #include "gernels/paged_cache.h"
 
 namespace gernels {

@@ -26,42 +26,4 @@ struct PagedCache {
     }
 };
 
-// Element types of keys, values and queries outside the cache.
-struct Bf16 {
-    static constexpr bool kBf16 = true;
-};
-struct F16 {
-    static constexpr bool kBf16 = false;
-};
-
-template<class T>
-__device__ __forceinline__ float half_to_float(uint32_t bits16) {
-    if constexpr (T::kBf16) {
-        return __builtin_bit_cast(float, bits16 << 16);
-    } else {
-        return (float)__builtin_bit_cast(_Float16, (unsigned short)bits16);
-    }
-}
-
-// Two values rounded to T (nearest even), the first in the low half.
-template<class T>
-__device__ __forceinline__ uint32_t pack_halves(float a, float b) {
-    if constexpr (T::kBf16) {
-        typedef __bf16 pair __attribute__((ext_vector_type(2)));
-        const pair p = {(__bf16)a, (__bf16)b};
-        return __builtin_bit_cast(uint32_t, p);
-    } else {
-        typedef _Float16 pair __attribute__((ext_vector_type(2)));
-        const pair p = {(_Float16)a, (_Float16)b};
-        return __builtin_bit_cast(uint32_t, p);
-    }
-}
-
-struct alignas(16) Words4 {
-    uint32_t w[4];
-};
-struct alignas(8) Words2 {
-    uint32_t w[2];
-};
-
 }  // namespace gernels

@@ -266,6 +266,21 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
                              float scale, int64_t max_queries, int64_t max_length, void *workspace,
                              int64_t workspace_bytes, void *stream);
 
+/* Y = X W^T for M (0 .. GERN_MATVEC4_MAX_ROWS) rows of X and W in 4 bits:
+ *   W[n, k] = scales[k / group, n] * (code[n, k] - zero[k / group, n])
+ * X: [M, K] in `type`, row stride ldx, 16-byte aligned; codes: [N, K / 2] bytes,
+ * the lower half of a byte is the even column, 16-byte aligned; scales:
+ * [K / group, N] in `type`; zeros: [K / group, N] bytes of 0 .. 255, or NULL: 8
+ * everywhere; Y: [M, N] in `type`, row stride ldy.  group is 32, 64 or 128 and
+ * divides K.  Sums are fp32, rounded once.  A row of X with an infinity gives
+ * NaN.  For more rows the products, and no longer the weights, are the work:
+ * that is gern_gemm_run's. */
+#define GERN_MATVEC4_MAX_ROWS 64
+int gern_matvec4_create(int64_t group, int type, int flags, gern_pipeline *out);
+int gern_matvec4_run(gern_pipeline p, const void *X, int64_t ldx, const uint8_t *codes, const void *scales,
+                     const uint8_t *zeros, void *Y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                     void *stream);
+
 /* What the kernels of the pipeline could not do and could only signal in
  * their results, since a run returns before they execute.  Waits for the
  * device, then stores in *count, and clears, the sum of

@@ -98,3 +98,21 @@ def attention(q, k, v, v_scales, limits, scale):
         o[i] = p @ v[:m]
         tol[i] = (2.0 ** -11 + 2 * exponent + (m / 32 + 16) * 2.0 ** -24) * (p @ np.abs(v[:m])) + 2.0 ** -25 * codes[:m].sum(axis=0) * (p * v_scales[:m]).max()
     return o, tol
+
+
+def matvec4(x, codes, scales, zeros, group, offset):
+    """x [m, k], codes [n, k / 2], scales and zeros [k / group, n].  Returns the result and how far fp32 sums may be from it
+    when they are taken of x (offset + q) and of x, group by group: a matrix instruction adds 32 products and its
+    accumulator, at most 8 roundings deep, group / 32 times; so does the sum of x, which counts offset + zero times; and
+    the groups' sums are added up, in eight parts."""
+    q = np.stack([codes & 15, codes >> 4], axis=2).reshape(codes.shape[0], -1).astype(np.float64)
+    y, tol = np.zeros((x.shape[0], codes.shape[0])), np.zeros((x.shape[0], codes.shape[0]))
+    size = np.zeros_like(y)
+    for g in range(scales.shape[0]):
+        part = slice(g * group, (g + 1) * group)
+        dots, sums = x[:, part] @ q[:, part].T, x[:, part].sum(axis=1, keepdims=True)
+        y += scales[g] * (dots - zeros[g] * sums)
+        most = np.abs(x[:, part]) @ (offset + q[:, part]).T + (offset + zeros[g]) * np.abs(x[:, part]).sum(axis=1, keepdims=True)
+        tol += np.abs(scales[g]) * (8 + group / 32) * 2.0 ** -24 * most
+        size += np.abs(scales[g]) * np.abs(dots - zeros[g] * sums)
+    return y, tol + (scales.shape[0] / 8 + 9) * 2.0 ** -24 * size
