@@ -174,18 +174,25 @@ __global__ void __launch_bounds__(THREADS) check_write_cache(gernels::NewTokensO
 template __global__ void check_write_cache<128, 16, 64, gernels::Bf16>(gernels::NewTokensOf<gernels::Bf16>, gernels::WritableCache);
 template __global__ void check_write_cache<64, 128, 256, gernels::F16>(gernels::NewTokensOf<gernels::F16>, gernels::WritableCache);
 
-template<int64_t D, int64_t PAGE, int64_t R, int64_t KEYS, class T>
-__global__ void __launch_bounds__(256) check_attend(gernels::AttentionBatchOf<T> batch, gernels::PagedCache cache, gernels::AttentionOut result) {
+template<int64_t D, int64_t PAGE, class T>
+__global__ void __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) check_attend_few(gernels::AttentionBatchOf<T> batch, gernels::PagedCache cache, gernels::AttentionOut result) {
     auto piece = result.piece(blockIdx.x, blockIdx.y, blockIdx.z);
-    gernels::attend<D, PAGE, R, 4, KEYS>(batch.whole(), cache.whole(), piece);
+    gernels::attend_few_rows<D, PAGE, 4>(batch.whole(), cache.whole(), piece);
 }
-template __global__ void check_attend<64, 32, 1, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<64, 32, 4, 0, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<128, 64, 1, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<128, 16, 2, 0, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<192, 16, 1, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<256, 16, 1, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend<256, 16, 1, 0, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template<int64_t D, int64_t PAGE, int64_t R, class T>
+__global__ void __launch_bounds__(256, 2) check_attend_many(gernels::AttentionBatchOf<T> batch, gernels::PagedCache cache, gernels::AttentionOut result) {
+    auto piece = result.piece(blockIdx.x, blockIdx.y, blockIdx.z);
+    gernels::attend_many_rows<D, PAGE, R, 4>(batch.whole(), cache.whole(), piece);
+}
+template __global__ void check_attend_few<64, 32, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_few<128, 64, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_few<128, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_few<192, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_few<256, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_many<64, 32, 4, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_many<128, 16, 2, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_many<192, 64, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_many<256, 16, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
 
 template<int64_t D, class T>
 __global__ void __launch_bounds__(256) check_join_splits(gernels::AttentionBatchOf<T> batch, gernels::JoinRows rows) {

@@ -37,9 +37,9 @@ public:
         return p;
     }
     // Compiles one more program of the pipeline.
-    int add(Composable program, int flags) {
+    int add(Composable program, int flags, int min_waves_per_simd = 0) {
         gern_pipeline_s one{};
-        const int rc = finish(&one, program, flags);
+        const int rc = finish(&one, program, flags, min_waves_per_simd);
         if (rc == 0) {
             const std::string name = one.runner ? one.runner->getKernelName() : one.kernel_name;
             p->variants.push_back({std::move(one.runner), one.source, name});
@@ -321,27 +321,41 @@ struct AttentionPlan {
     int64_t row_tiles, splits, chunk;
 };
 
-constexpr int64_t kMaxSplits = 64;  // gernels/cache_attention.h, join_splits
+constexpr int64_t kMaxSplits = 256;  // gernels/cache_attention.h, join_splits
 
-// Row tiles per wavefront of the program that divides rows among wavefronts: accumulators and queries of R
-// tiles take 3/8 R D registers a lane.
+// The programs of a pipeline, four wavefronts a workgroup: few rows (queries times the heads that share a head of the
+// cache) against keys that the wavefronts divide, or many rows divided among the wavefronts.
+constexpr int64_t kAttentionWaves = 4;
+
+// 16-row tiles of a wavefront of the second: accumulators and queries take 3/8 R D registers a lane, and two
+// wavefronts are to fit a SIMD.
 int64_t attentionRowTiles(int64_t head_dim) {
-    return head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;
+    return head_dim <= 128 ? 2 : 1;
+}
+
+// Wavefronts of the first that its registers leave room for on a SIMD.
+int attentionResidentWaves(int64_t head_dim) {
+    return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2;
 }
 
 AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, int64_t rows, int64_t max_length) {
     AttentionPlan plan{};
-    // Up to 32 rows (queries times the heads that share a head of the cache) the wavefronts of a workgroup divide
-    // the keys, beyond that the rows.
     plan.variant = rows <= 32 ? 0 : 1;
-    const int64_t tile = plan.variant == 0 ? 16 : 64 * attentionRowTiles(head_dim);
+    const int64_t tile = plan.variant == 0 ? 16 : 16 * kAttentionWaves * attentionRowTiles(head_dim);
     plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
-    // Keys are split until there are four workgroups for each of 256 CUs, into pieces of at least 256 keys.
+    // Keys are split, into pieces of at least 256, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
+    // to three times what is resident, so that requests of different lengths leave few CUs idle at the end.  Few rows of
+    // more than 128 dimensions: two, what is resident, because the joined parts are larger and a start costs more.
+    // Measured (us) with 512 / 1024 / 2048 / 4096: 64 requests of 4096 to 8192 keys, 8 heads of 128: 181 / 175 / 155 /
+    // 165; 3 of 131072 to 262144: 266 / 188 / 184 / 197; 32 of 1250 to 2500, 16 heads of 256: 95 / 110 / 109 / -; 6 of 113
+    // to 447 queries and 4032 to 5915 keys, 4 heads of 64 for 16: 166 / 124 / 116 / -.
+    const int64_t wanted = plan.variant == 0 && head_dim > 128 ? 512 : 2048;
     const int64_t whole = requests * heads * plan.row_tiles;
-    const int64_t wanted = std::max<int64_t>(1, (1024 + whole - 1) / whole);
-    const int64_t chunk = std::max<int64_t>(256, (max_length + wanted - 1) / wanted);
-    plan.chunk = std::max((chunk + 127) / 128 * 128, (max_length + kMaxSplits * 128 - 1) / (kMaxSplits * 128) * 128);
+    const int64_t splits = std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
+    plan.chunk = std::max<int64_t>(256, ((max_length + splits - 1) / splits + 255) / 256 * 256);
     plan.splits = std::max<int64_t>(1, (max_length + plan.chunk - 1) / plan.chunk);
+    // BLOCK_Y holds 65535 pieces; a workgroup takes further row tiles in turn
+    plan.row_tiles = std::min(plan.row_tiles, 65535 / plan.splits);
     return plan;
 }
 
@@ -384,28 +398,35 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
         const std::string header = "gernels/cache_attention.h", batch_type = "gernels::AttentionBatchOf<" + typeName(type) + ">";
         AbstractDataTypePtr batch(new const annot::WholeADT("batch", batch_type));
         AbstractDataTypePtr cache(new const annot::WholeADT("cache", "gernels::PagedCache"));
-        for (bool keys : {true, false}) {
+        for (bool few : {true, false}) {
             using Out = hip::AttentionOut;
             AbstractDataTypePtr result(new const annot::PiecesADT<Out>("result", "gernels::AttentionOut", "piece",
                                                                       {{"pieces", &Out::pieces}, {"heads", &Out::heads}, {"requests", &Out::requests}}));
-            annot::PieceFunction attend("gernels::attend", header, {batch, cache}, result, {"pieces", "heads", "requests"},
-                                        {"head_dim", "page", "row_tiles", "waves", "divide_keys"});
+            const std::vector<std::string> constants = few ? std::vector<std::string>{"head_dim", "page", "waves"} :
+                                                             std::vector<std::string>{"head_dim", "page", "row_tiles", "waves"};
+            annot::PieceFunction attend(few ? "gernels::attend_few_rows" : "gernels::attend_many_rows", header, {batch, cache}, result,
+                                        {"pieces", "heads", "requests"}, constants);
+            std::map<std::string, Variable> bound{constant("head_dim", head_dim), constant("page", page_size), constant("waves", kAttentionWaves)};
+            if (!few) {
+                bound.insert(constant("row_tiles", attentionRowTiles(head_dim)));
+            }
             Variable x("x"), head("head"), request("request"), threads("threads");
+            // Heads along BLOCK_X: the workgroups that run together read the heads of the same pages, which stand side by
+            // side (3 requests of 131072 to 262144 keys: 222 us with the pieces of the keys along BLOCK_X, 188 so).
             Composable program = Global(
-                (Tile(result["pieces"], x.bind(1)) || Grid::BLOCK_X)((Tile(result["heads"], head.bind(1)) || Grid::BLOCK_Y)(
-                    (Tile(result["requests"], request.bind(1)) || Grid::BLOCK_Z)(
-                        attend[{constant("head_dim", head_dim), constant("page", page_size), constant("row_tiles", keys ? 1 : attentionRowTiles(head_dim)),
-                                constant("waves", 4), constant("divide_keys", keys)}](batch, cache, result)))),
-                {{Grid::BLOCK_DIM_X, threads.bind(256)}});
-            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                (Tile(result["pieces"], x.bind(1)) || Grid::BLOCK_Y)((Tile(result["heads"], head.bind(1)) || Grid::BLOCK_X)(
+                    (Tile(result["requests"], request.bind(1)) || Grid::BLOCK_Z)(attend[bound](batch, cache, result)))),
+                {{Grid::BLOCK_DIM_X, threads.bind(64 * kAttentionWaves)}});
+            // two wavefronts of the second program on a SIMD, where its staged keys leave room in LDS
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP, few ? attentionResidentWaves(head_dim) : head_dim <= 128 ? 2 : 1) != 0) {
                 return 1;
             }
         }
         using Rows = hip::JoinRows;
-        AbstractDataTypePtr rows(new const annot::PiecesADT<Rows>("rows", "gernels::JoinRows", "block", {{"blocks", &Rows::blocks}}));
-        annot::PieceFunction join("gernels::join_splits", header, {batch}, rows, {"blocks"}, {"head_dim", "waves"});
+        AbstractDataTypePtr rows(new const annot::PiecesADT<Rows>("rows", "gernels::JoinRows", "block", {{"rows", &Rows::rows}}));
+        annot::PieceFunction join("gernels::join_splits", header, {batch}, rows, {"rows"}, {"head_dim", "waves"});
         Variable x("x"), threads("threads");
-        Composable program = Global((Tile(rows["blocks"], x.bind(1)) || Grid::BLOCK_X)(
+        Composable program = Global((Tile(rows["rows"], x.bind(1)) || Grid::BLOCK_X)(
                                         join[{constant("head_dim", head_dim), constant("waves", 4)}](batch, rows)),
                                     {{Grid::BLOCK_DIM_X, threads.bind(256)}});
         if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0 || p.addFaultCount("gern_cache_attention_create") != 0) {
@@ -484,7 +505,7 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     if (rc != 0 || plan.splits == 1) {
         return rc;
     }
-    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, (rows + 3) / 4};
+    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows};
     const int joined = evaluate(p, 2, who, stream, {{"batch", &batch}, {"rows", &join}});
     p->last_variant = plan.variant;
     return joined;

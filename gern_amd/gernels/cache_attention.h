@@ -33,8 +33,9 @@
 // 2^-11 of a weight) because fp16 holds every e4m3 code exactly, and their sum is
 // taken before rounding; bf16 weights would cost eight times that error.
 //
-// Bound by memory for few queries: 2 D bytes a key and head, read once.  Codes
-// are loaded one 32-key step ahead, page numbers two.
+// Bound by memory for few queries: 2 D bytes a key and head, read once (64 requests of
+// 4096 to 8192 keys, 8 heads of 128: 788 MB in 155 us, 5.1 TB/s; a copy of 1 GiB
+// moves 5.2 on the same GPU).
 #pragma once
 
 #include "gernels/half_tiles.h"
@@ -108,17 +109,69 @@ __device__ __forceinline__ float sum_over_lane_groups(float x) {
     return over_lane_groups(x, [](float a, float b) { return a + b; });
 }
 
+// 0, as a value that may differ from lane to lane for all the compiler knows.
+__device__ __forceinline__ int opaque_zero() {
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    return zero;
+}
+
 // Below every score; finite, so that a row that has seen nothing yet gives 2^(-inf - m) = 0.
 constexpr float kLowest = -1.0e30f;
 
-// 32 keys of one head of the cache: two tiles of 16, each inside a page.
+// 16 keys of one head of the cache, as they are in memory.
 template<int D>
-struct KeyTile {
-    uint32_t k[2][D / 16];  // lane (g, c): key c of tile t, dimensions [g D/4, (g+1) D/4)
-    uint32_t v[8][D / 64];  // lane (g, c): key 4g + j of tile j / 4, dimensions [c D/16, (c+1) D/16)
-    float k_scale[2], v_scale[2];
-    bool there[2];          // the tile's page is in the cache
+struct RawKeys {
+    uint32_t k[D / 16];     // lane (g, c): key c, dimensions [g D/4, (g+1) D/4)
+    uint32_t v[4][D / 64];  // lane (g, c): keys 4g .. 4g+3, dimensions [c D/16, (c+1) D/16)
+    float k_scale, v_scale;
+    int64_t at;             // its page and head
+    bool there;             // it has keys, and their page is in the cache
+
+    // Fragment i of K: dimensions [32 i, 32 i + 32) in the order described above.
+    template<bool BF16>
+    __device__ __forceinline__ Frag key_frag(int i) const {
+        const uint32_t a = k[2 * i], b = k[2 * i + 1];
+        return {{codes_to_halves<BF16, false>(a), codes_to_halves<BF16, true>(a), codes_to_halves<BF16, false>(b), codes_to_halves<BF16, true>(b)}};
+    }
+    // Half of fragment i of V^T: dimension c D/16 + i of keys 4g .. 4g+3.
+    __device__ __forceinline__ Words2 value_half(int i) const {
+        const uint32_t a = v[0][i / 4], b = v[1][i / 4], c = v[2][i / 4], d = v[3][i / 4];
+        // v_perm_b32: selector bytes 0-3 pick from the second operand, 4-7 from the first
+        const uint32_t pick = i % 4 < 2 ? 0x05010400u : 0x07030602u;
+        const uint32_t ab = __builtin_amdgcn_perm(b, a, pick), cd = __builtin_amdgcn_perm(d, c, pick);
+        const uint32_t column = __builtin_amdgcn_perm(cd, ab, i % 2 == 0 ? 0x05040100u : 0x07060302u);
+        return {{codes_to_halves<false, false>(column), codes_to_halves<false, true>(column)}};
+    }
+    // What stands behind the last key may be anything, NaN too, and 0 * NaN must not reach a sum.
+    __device__ __forceinline__ void clear_values_behind(int base, int length) {
+        const int g = lane_id() / 16;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const bool keep = there && base + 4 * g + j < length;
+#pragma unroll
+            for (int w = 0; w < D / 64; w++) {
+                v[j][w] = keep ? v[j][w] : 0u;
+            }
+        }
+    }
 };
+
+// The scales of a tile as the softmax takes them.
+struct TileScales {
+    float k;      // of the scores, with the attention's own scale
+    float up;     // log2 of the values' scale
+    float per_v;  // one over it
+    bool there;
+};
+template<int D>
+__device__ __forceinline__ TileScales scales_of(const RawKeys<D> &tile, float scale) {
+    // A scale of values under 2^-64 counts as that: its codes are zero, or too small to matter.  The scale of the
+    // scores stays above zero because -infinity, a key that is not seen, is multiplied by it.
+    const float k = tile.k_scale * scale, v = tile.v_scale;
+    const float vs = !tile.there ? 1.0f : v < 5.421010862e-20f ? 5.421010862e-20f : v;
+    return {!tile.there ? 1.0f : k < 1.0e-30f ? 1.0e-30f : k, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
+}
 
 // What a wavefront needs to walk the keys of one request and head.
 template<int D, int PAGE>
@@ -126,35 +179,37 @@ struct KeyWalk {
     const PagedCache &cache;
     const int32_t *pages;  // the request's row of the block table
     int64_t head;
+    int width;             // of the table
     int length;            // keys in the cache
+    int zero;
 
-    // Page numbers of the two tiles at key `base` (uniform); -1 behind the last key.
-    __device__ __forceinline__ void look_up(int base, int id[2]) const {
+    // The page number at key `base` (uniform; behind the table the last one).  Does not wait for `length`.  The load is a vector
+    // load (`zero` is a 0 that the compiler does not see through), in order with those of the codes: a scalar load is
+    // put where its value is needed and waited for there.
+    __device__ __forceinline__ int look_up(int base) const {
+        return pages[min(base / PAGE, width - 1) + zero];
+    }
+    // The 16 keys at `base`, a multiple of 16, in two halves.  Every address is inside a whole page of the cache: what
+    // is not there is read from page 0.
+    __device__ __forceinline__ void load_keys(RawKeys<D> &tile, int base, int looked_up) const {
+        const int lane = lane_id(), g = lane / 16, c = lane % 16;
+        const int id = __builtin_amdgcn_readfirstlane(looked_up);
+        tile.there = id >= 0 && id < cache.pages && base < length;
+        tile.at = (int64_t)(tile.there ? id : 0) * cache.heads + head;
+        tile.k_scale = cache.k_scales[tile.at + zero];
+        tile.v_scale = cache.v_scales[tile.at + zero];
+        const uint32_t *k = cache.k + tile.at * (PAGE * D / 4) + (base % PAGE + c) * (D / 4) + g * (D / 16);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            id[t] = base + 16 * t < length ? pages[(base + 16 * t) / PAGE] : -1;
+        for (int i = 0; i < D / 64; i++) {
+            load_words<4>(&tile.k[4 * i], k + 4 * i);
         }
     }
-    // Every address is inside a whole page of the cache: what is not there is read from page 0.
-    __device__ __forceinline__ void load(KeyTile<D> &tile, int base, const int id[2]) const {
+    __device__ __forceinline__ void load_values(RawKeys<D> &tile, int base) const {
         const int lane = lane_id(), g = lane / 16, c = lane % 16;
+        const uint32_t *v = cache.v + tile.at * (PAGE * D / 4) + (base % PAGE + 4 * g) * (D / 4) + c * (D / 64);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            tile.there[t] = id[t] >= 0 && id[t] < cache.pages;
-            const int64_t at = (int64_t)(tile.there[t] ? id[t] : 0) * cache.heads + head;
-            const int place = (base + 16 * t) % PAGE;
-            const uint32_t *k = cache.k + at * (PAGE * D / 4) + (place + c) * (D / 4) + g * (D / 16);
-            const uint32_t *v = cache.v + at * (PAGE * D / 4) + (place + 4 * g) * (D / 4) + c * (D / 64);
-#pragma unroll
-            for (int i = 0; i < D / 64; i++) {
-                load_words<4>(&tile.k[t][4 * i], k + 4 * i);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                load_words<D / 64>(tile.v[4 * t + j], v + j * (D / 4));
-            }
-            tile.k_scale[t] = cache.k_scales[at];
-            tile.v_scale[t] = cache.v_scales[at];
+        for (int j = 0; j < 4; j++) {
+            load_words<D / 64>(tile.v[j], v + j * (D / 4));
         }
     }
 };
@@ -179,9 +234,11 @@ struct RowState {
         }
     }
 
-    // Adds the keys [base, base + 32).  `whole`: every row sees all of them.
-    __device__ __forceinline__ void add(KeyTile<D> &tile, int base, int length, bool whole, float scale) {
-        const int lane = lane_id(), g = lane / 16;
+    // Adds the keys [base, base + 32): fragment i of 16-key tile t is key_frag(t, i), of V^T value_frag(i).
+    // `whole`: every row sees all of them.  after_keys() is called when the keys' fragments have been used.
+    template<class KeyFrag, class AfterKeys, class Scales, class ValueFrag>
+    __device__ __forceinline__ void add(int base, bool whole, KeyFrag key_frag, Scales scales_of_tile, AfterKeys after_keys, ValueFrag value_frag) {
+        const int g = lane_id() / 16;
         f32x4 s[R][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -191,45 +248,32 @@ struct RowState {
             }
 #pragma unroll
             for (int i = 0; i < D / 32; i++) {
-                const uint32_t a = tile.k[t][2 * i], b = tile.k[t][2 * i + 1];
-                const Frag k = {{codes_to_halves<BF16, false>(a), codes_to_halves<BF16, true>(a), codes_to_halves<BF16, false>(b),
-                                 codes_to_halves<BF16, true>(b)}};
+                const Frag k = key_frag(t, i);
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     s[r][t] = mfma_16x16x32<BF16>(k, q[r][i], s[r][t]);
                 }
             }
         }
-        float up[2], per_v[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            // a scale under 2^-64 counts as that (its codes are zero, or too small to matter)
-            float vs = tile.v_scale[t] < 5.421010862e-20f ? 5.421010862e-20f : tile.v_scale[t];
-            vs = whole || (tile.there[t] && base + 16 * t < length) ? vs : 1.0f;
-            up[t] = __builtin_amdgcn_logf(vs);  // base 2
-            per_v[t] = __builtin_amdgcn_rcpf(vs);
-        }
+        const TileScales scales[2] = {scales_of_tile(0), scales_of_tile(1)};
+        after_keys();
         Frag p[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float y[8];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const float ks = tile.k_scale[t] * scale;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    y[4 * t + e] = __builtin_fmaf(s[r][t][e], ks, up[t]);
-                }
-            }
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const bool seen = tile.there[j / 4] && base + 16 * (j / 4) + 4 * g + j % 4 < limit[r];
-                    y[j] = seen ? y[j] : -__builtin_inff();
+                    const bool seen = scales[j / 4].there && base + 16 * (j / 4) + 4 * g + j % 4 < limit[r];
+                    s[r][j / 4][j % 4] = seen ? s[r][j / 4][j % 4] : -__builtin_inff();
                 }
             }
-            float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y[0], y[1]), __builtin_fmaxf(y[2], y[3])),
-                                        __builtin_fmaxf(__builtin_fmaxf(y[4], y[5]), __builtin_fmaxf(y[6], y[7])));
+            // scales are not negative: the largest product of a tile is its largest score
+            float top = kLowest;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const float most = __builtin_fmaxf(__builtin_fmaxf(s[r][t][0], s[r][t][1]), __builtin_fmaxf(s[r][t][2], s[r][t][3]));
+                top = __builtin_fmaxf(top, __builtin_fmaf(most, scales[t].k, scales[t].up));
+            }
             top = max_over_lane_groups(top);
             if (__ballot(top > m[r]) != 0) {
                 const float now = __builtin_fmaxf(top, m[r]);
@@ -241,49 +285,27 @@ struct RowState {
                     o[r][i] *= shrink;
                 }
             }
+            float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                y[j] = __builtin_amdgcn_exp2f(y[j] - m[r]);
-                l[r] = __builtin_fmaf(y[j], per_v[j / 4], l[r]);
+            for (int t = 0; t < 2; t++) {
+                const float shift = scales[t].up - m[r];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    y[4 * t + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][e], scales[t].k, shift));
+                    l[r] = __builtin_fmaf(y[4 * t + e], scales[t].per_v, l[r]);
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 p[r].w[j] = pack_halves<F16>(y[2 * j], y[2 * j + 1]);
             }
         }
-        if (!whole) {
-            // what stands behind the last key may be anything, NaN too: 0 * NaN must not reach the sum
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const bool keep = tile.there[j / 4] && base + 16 * (j / 4) + 4 * g + j % 4 < length;
+        for (int i = 0; i < D / 16; i++) {
+            const Frag v = value_frag(i);
 #pragma unroll
-                for (int w = 0; w < D / 64; w++) {
-                    tile.v[j][w] = keep ? tile.v[j][w] : 0u;
-                }
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < D / 64; w++) {
-            uint32_t column[2][4];  // [tile][byte of the word]: four keys of one dimension
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t a = tile.v[4 * t][w], b = tile.v[4 * t + 1][w], c = tile.v[4 * t + 2][w], d = tile.v[4 * t + 3][w];
-                // v_perm_b32: selector bytes 0-3 pick from the second operand, 4-7 from the first
-                const uint32_t ab_low = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_high = __builtin_amdgcn_perm(b, a, 0x07030602u);
-                const uint32_t cd_low = __builtin_amdgcn_perm(d, c, 0x05010400u), cd_high = __builtin_amdgcn_perm(d, c, 0x07030602u);
-                column[t][0] = __builtin_amdgcn_perm(cd_low, ab_low, 0x05040100u);
-                column[t][1] = __builtin_amdgcn_perm(cd_low, ab_low, 0x07060302u);
-                column[t][2] = __builtin_amdgcn_perm(cd_high, ab_high, 0x05040100u);
-                column[t][3] = __builtin_amdgcn_perm(cd_high, ab_high, 0x07060302u);
-            }
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const Frag v = {{codes_to_halves<false, false>(column[0][b]), codes_to_halves<false, true>(column[0][b]),
-                                 codes_to_halves<false, false>(column[1][b]), codes_to_halves<false, true>(column[1][b])}};
-#pragma unroll
-                for (int r = 0; r < R; r++) {
-                    o[r][4 * w + b] = mfma_16x16x32<false>(v, p[r], o[r][4 * w + b]);
-                }
+            for (int r = 0; r < R; r++) {
+                o[r][i] = mfma_16x16x32<false>(v, p[r], o[r][i]);
             }
         }
     }
@@ -320,212 +342,358 @@ __device__ __forceinline__ void store_floats(float *to, const float (&x)[N]) {
     }
 }
 
+// What a workgroup knows of its request, and the rows and keys of its piece.
+template<int D, int PAGE, class T>
+struct AttentionRequest {
+    int first, queries, length;  // first row of q, rows, keys
+    int group, rows;             // rows * group: rows of this head of the cache
+    int split, splits;
+    int64_t all_rows;
+
+    __device__ __forceinline__ AttentionRequest(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
+        const int tokens = (int)batch.tokens;
+        first = min(max(batch.starts[piece.request], 0), tokens);
+        queries = min(max(batch.starts[piece.request + 1], first), tokens) - first;
+        const int64_t room = batch.width * PAGE;
+        const int asked = batch.lengths[piece.request];
+        length = (int)min((int64_t)max(asked, 0), room);
+        group = (int)batch.group;
+        rows = queries * group;
+        splits = (int)piece.to.splits;
+        split = (int)piece.x % splits;
+        all_rows = batch.tokens * piece.to.heads * group;
+        if (asked > room && piece.x == 0 && piece.head == 0 && threadIdx.x == 0) {
+            atomicAdd(cache.faults, 1u);
+        }
+    }
+    // Keys that a row sees.
+    __device__ __forceinline__ int limit(int row) const {
+        return min(max(length - queries + row / group + 1, 0), length);
+    }
+    // Where a row's result, or its part of split `split`, is.
+    __device__ __forceinline__ int64_t token(int row) const {
+        return first + row / group;
+    }
+    __device__ __forceinline__ int64_t head(int row, const AttentionPiece &piece) const {
+        return piece.head * group + row % group;
+    }
+    __device__ __forceinline__ int64_t part(int row, const AttentionPiece &piece) const {
+        return split * all_rows + token(row) * (piece.to.heads * group) + head(row, piece);
+    }
+};
+
+// Queries and limits of the R tiles of rows from row0 on.
+template<int D, int PAGE, int R, class T>
+__device__ __forceinline__ void load_queries(RowState<D, R, T::kBf16> &state, const AttentionRequest<D, PAGE, T> &request, const AttentionBatchOf<T> &batch,
+                                             const AttentionPiece &piece, int row0) {
+    const int lane = lane_id(), g = lane / 16, c = lane % 16;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = row0 + 16 * r + c;
+        const bool mine = row < request.rows;
+        state.limit[r] = mine ? request.limit(row) : 0;
+        const uint32_t *q = batch.q + request.token(mine ? row : 0) * batch.q_pitch + request.head(mine ? row : 0, piece) * (D / 2) + g * (D / 8);
+#pragma unroll
+        for (int s = 0; s < D / 32; s++) {
+            load_words<4>(state.q[r][s].w, q + 4 * s);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                // the scale's sign goes to the queries
+                state.q[r][s].w[w] = mine ? state.q[r][s].w[w] ^ (batch.scale < 0.0f ? 0x80008000u : 0u) : 0u;
+            }
+        }
+    }
+}
+
 }  // namespace detail
 
-// One piece: R tiles of 16 query rows (a row is a query and one of the G heads
-// that share a head of the cache) against one split of the keys, on WAVES
-// wavefronts.  KEYS: the wavefronts take the 32-key tiles in turn and meet in LDS
-// at the end; otherwise each takes R row tiles of its own and all walk the same
-// keys, which then come from the CU's cache for all but the first.
-template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, int64_t KEYS, class T>
-__device__ __forceinline__ void attend(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
-    constexpr int kRows = 16 * R;                            // of a wavefront
-    constexpr int kTileRows = KEYS ? kRows : kRows * WAVES;  // of a workgroup
-    constexpr bool kBf16 = T::kBf16;
+// One piece for FEW rows (a row is a query and one of the G heads that share a head
+// of the cache): 16 of them against one split of the keys.  The WAVES wavefronts
+// take the 32-key tiles in turn, each from memory to its registers, and meet in
+// LDS at the end.
+template<int64_t D, int64_t PAGE, int64_t WAVES, class T>
+__device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
     const AttentionOut &to = piece.to;
     const int lane = lane_id(), g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    const int splits = (int)to.splits, split = (int)piece.x % splits, tiles = (int)to.pieces / splits;
-    const int group = (int)batch.group;
+    const detail::AttentionRequest<D, PAGE, T> request(batch, cache, piece);
+    const detail::KeyWalk<D, PAGE> walk = {cache, batch.table + piece.request * batch.width, piece.head, (int)batch.width, request.length, detail::opaque_zero()};
+    const int tiles = (int)to.pieces / request.splits;
 
-    const int tokens = (int)batch.tokens;
-    const int first = min(max(batch.starts[piece.request], 0), tokens);
-    const int queries = min(max(batch.starts[piece.request + 1], first), tokens) - first;
-    const int64_t room = batch.width * PAGE;
-    const int asked = batch.lengths[piece.request];
-    const int length = (int)min((int64_t)max(asked, 0), room);
-    const int rows = queries * group;
-    if (asked > room && piece.x == 0 && piece.head == 0 && threadIdx.x == 0) {
-        atomicAdd(cache.faults, 1u);
-    }
-    const detail::KeyWalk<D, PAGE> walk = {cache, batch.table + piece.request * batch.width, piece.head, length};
-    const int64_t all_rows = batch.tokens * to.heads * group;
-
-    for (int tile = (int)piece.x / splits; tile * kTileRows < rows; tile += tiles) {
-        const int row0 = tile * kTileRows + (KEYS ? 0 : wave * kRows);
-        detail::RowState<D, R, kBf16> state;
+    for (int tile = (int)piece.x / request.splits; tile * 16 < request.rows; tile += tiles) {
+        const int row0 = tile * 16;
+        detail::RowState<D, 1, T::kBf16> state;
         state.clear();
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int row = row0 + 16 * r + c;
-            const int i = row / group, u = row % group;
-            state.limit[r] = row < rows ? min(max(length - queries + i + 1, 0), length) : 0;
-            const uint32_t *q = batch.q + (first + (row < rows ? i : 0)) * batch.q_pitch + (piece.head * group + (row < rows ? u : 0)) * (D / 2) + g * (D / 8);
-#pragma unroll
-            for (int s = 0; s < D / 32; s++) {
-                detail::load_words<4>(state.q[r][s].w, q + 4 * s);
-                if (row >= rows) {
-                    state.q[r][s] = detail::Frag{{0u, 0u, 0u, 0u}};
-                }
-            }
-        }
-        // keys that any / every row of this wavefront sees
-        const int last_row = min(row0 + kRows, rows) - 1;
-        const int most = row0 < rows ? min(max(length - queries + last_row / group + 1, 0), length) : 0;
-        const int least = row0 + kRows <= rows ? min(max(length - queries + row0 / group + 1, 0), length)
-                                               : min(most, max(length - queries + row0 / group + 1, 0));
-        const int64_t begin64 = (int64_t)split * to.chunk;
-        const int begin = (int)min(begin64, (int64_t)most);
-        const int end = split + 1 < splits ? (int)min(begin64 + to.chunk, (int64_t)most) : most;
-        constexpr int kStep = KEYS ? 32 * WAVES : 32;
+        detail::load_queries(state, request, batch, piece, row0);
+        // keys that any / every row sees (rows behind the last one are not stored)
+        const int most = request.limit(min(row0 + 16, request.rows) - 1), least = request.limit(row0);
+        const int64_t begin = (int64_t)request.split * to.chunk;
+        // `end` cuts a tile only where no row sees further: splits are whole tiles
+        const int end = request.split + 1 < request.splits ? (int)min(begin + to.chunk, (int64_t)most) : most;
+        constexpr int kStep = 32 * WAVES;
         bool missing = false;
-
-        auto add = [&](detail::KeyTile<D> &keys, int base) {
-            // `end` cuts a tile only where no row sees further: splits are whole tiles
-            const bool whole = base + 32 <= least && keys.there[0] && keys.there[1];
-            missing = missing || (!keys.there[0] && base < end) || (!keys.there[1] && base + 16 < end);
-            state.add(keys, base, length, whole, batch.scale);
-        };
-        int base = begin + (KEYS ? 32 * wave : 0);
+        // Keys of the next step are loaded when this step's have been multiplied, values likewise, page numbers a step
+        // before: no register is held for a load that waits, and none of the loads is waited for where it is issued.
+        int base = (int)min(begin, (int64_t)most) + 32 * wave;
+        detail::RawKeys<D> keys[2];
+        int id[2] = {walk.look_up(base), walk.look_up(base + 16)};
         if (base < end) {
-            detail::KeyTile<D> even, odd;
-            int id[2], next_id[2];
-            walk.look_up(base, id);
-            walk.look_up(base + kStep, next_id);
-            walk.load(even, base, id);
-            while (true) {
-                if (base + kStep < end) {
-                    walk.load(odd, base + kStep, next_id);
-                    walk.look_up(base + 2 * kStep, next_id);
-                }
-                add(even, base);
-                base += kStep;
-                if (base >= end) {
-                    break;
-                }
-                if (base + kStep < end) {
-                    walk.load(even, base + kStep, next_id);
-                    walk.look_up(base + 2 * kStep, next_id);
-                }
-                add(odd, base);
-                base += kStep;
-                if (base >= end) {
-                    break;
-                }
+            walk.load_keys(keys[0], base, id[0]);
+            walk.load_keys(keys[1], base + 16, id[1]);
+            id[0] = walk.look_up(base + kStep);
+            id[1] = walk.look_up(base + kStep + 16);
+            walk.load_values(keys[0], base);
+            walk.load_values(keys[1], base + 16);
+        }
+        while (base < end) {
+            const bool there[2] = {keys[0].there, keys[1].there};
+            const bool whole = base + 32 <= least && there[0] && there[1];
+            missing = missing || !there[0] || (!there[1] && base + 16 < end);
+            const bool more = base + kStep < end;
+            state.add(
+                base, whole, [&](int t, int i) { return keys[t].template key_frag<T::kBf16>(i); },
+                [&](int t) { return detail::scales_of(keys[t], __builtin_fabsf(batch.scale)); },
+                [&]() {
+                    if (!whole) {
+                        keys[0].clear_values_behind(base, request.length);
+                        keys[1].clear_values_behind(base + 16, request.length);
+                    }
+                    if (more) {
+                        walk.load_keys(keys[0], base + kStep, id[0]);
+                        walk.load_keys(keys[1], base + kStep + 16, id[1]);
+                        id[0] = walk.look_up(base + 2 * kStep);
+                        id[1] = walk.look_up(base + 2 * kStep + 16);
+                    }
+                },
+                [&](int i) {
+                    const Words2 a = keys[0].value_half(i), b = keys[1].value_half(i);
+                    return detail::Frag{{a.w[0], a.w[1], b.w[0], b.w[1]}};
+                });
+            if (more) {
+                walk.load_values(keys[0], base + kStep);
+                walk.load_values(keys[1], base + kStep + 16);
             }
+            base += kStep;
         }
         if (missing && lane == 0) {
             atomicAdd(cache.faults, 1u);
         }
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            state.l[r] = detail::sum_over_lane_groups(state.l[r]);
-        }
+        state.l[0] = detail::sum_over_lane_groups(state.l[0]);
 
-        if constexpr (KEYS != 0) {
-            // The wavefronts' parts meet in LDS; thread t then takes D / 16 values of row t / 16.
-            constexpr int kPitch = D + 4;
-            constexpr int kPart = D / 16;
-            __shared__ __attribute__((aligned(16))) float parts[WAVES][16][kPitch];
-            __shared__ float part_m[WAVES][16], part_l[WAVES][16];
-            static_assert(WAVES == 4, "256 threads share 16 rows");
+        // The wavefronts' parts meet in LDS; thread t then takes D / 16 values of row t / 16.
+        constexpr int kPitch = D + 4;
+        constexpr int kPart = D / 16;
+        __shared__ __attribute__((aligned(16))) float parts[WAVES][16][kPitch];
+        __shared__ float part_m[WAVES][16], part_l[WAVES][16];
+        static_assert(WAVES >= 4, "256 threads share 16 rows");
+        __syncthreads();  // the previous rows have been read
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                __syncthreads();  // the previous rows have been read
+        for (int e = 0; e < 4; e++) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
+            for (int i = 0; i < D / 16; i += 4) {
+                const float x[4] = {state.o[0][i][e], state.o[0][i + 1][e], state.o[0][i + 2][e], state.o[0][i + 3][e]};
+                detail::store_floats(&parts[wave][c][g * (D / 4) + e * (D / 16) + i], x);
+            }
+        }
+        if (g == 0) {
+            part_m[wave][c] = state.m[0];
+            part_l[wave][c] = state.l[0];
+        }
+        __syncthreads();
+        const int at = threadIdx.x / 16, d = (threadIdx.x % 16) * kPart, row = row0 + at;
+        if (threadIdx.x < 256 && row < request.rows) {
+            float m = part_m[0][at];
 #pragma unroll
-                    for (int i = 0; i < D / 16; i += 4) {
-                        const float x[4] = {state.o[r][i][e], state.o[r][i + 1][e], state.o[r][i + 2][e], state.o[r][i + 3][e]};
-                        detail::store_floats(&parts[wave][c][g * (D / 4) + e * (D / 16) + i], x);
-                    }
-                }
-                if (g == 0) {
-                    part_m[wave][c] = state.m[r];
-                    part_l[wave][c] = state.l[r];
-                }
-                __syncthreads();
-                const int at = threadIdx.x / 16, d = (threadIdx.x % 16) * kPart;
-                const int row = row0 + 16 * r + at;
-                float m = part_m[0][at];
+            for (int w = 1; w < WAVES; w++) {
+                m = __builtin_fmaxf(m, part_m[w][at]);
+            }
+            float sum = 0.0f, x[kPart];
 #pragma unroll
-                for (int w = 1; w < WAVES; w++) {
-                    m = __builtin_fmaxf(m, part_m[w][at]);
-                }
-                float sum = 0.0f, x[kPart];
+            for (int i = 0; i < kPart; i++) {
+                x[i] = 0.0f;
+            }
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float weight = __builtin_amdgcn_exp2f(part_m[w][at] - m);
+                sum = __builtin_fmaf(part_l[w][at], weight, sum);
 #pragma unroll
                 for (int i = 0; i < kPart; i++) {
-                    x[i] = 0.0f;
-                }
-#pragma unroll
-                for (int w = 0; w < WAVES; w++) {
-                    const float weight = __builtin_amdgcn_exp2f(part_m[w][at] - m);
-                    sum = __builtin_fmaf(part_l[w][at], weight, sum);
-#pragma unroll
-                    for (int i = 0; i < kPart; i++) {
-                        x[i] = __builtin_fmaf(parts[w][at][d + i], weight, x[i]);
-                    }
-                }
-                if (row < rows) {
-                    const int64_t token = first + row / group, head = piece.head * group + row % group;
-                    if (splits == 1) {
-                        const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-                        for (int i = 0; i < kPart; i++) {
-                            x[i] *= per_sum;
-                        }
-                        detail::store_halves<T>(to.out + token * to.out_pitch + head * (D / 2), d, x);
-                    } else {
-                        const int64_t slot = split * all_rows + token * (to.heads * group) + head;
-                        detail::store_floats(to.partial + slot * D + d, x);
-                        if (d == 0) {
-                            to.stats[2 * slot] = m;
-                            to.stats[2 * slot + 1] = sum;
-                        }
-                    }
+                    x[i] = __builtin_fmaf(parts[w][at][d + i], weight, x[i]);
                 }
             }
-        } else {
+            if (request.splits == 1) {
+                const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int row = row0 + 16 * r + c;
-                if (row < rows) {
-                    const int64_t token = first + row / group, head = piece.head * group + row % group;
-                    const float per_sum = splits > 1 ? 1.0f : state.l[r] != 0.0f ? 1.0f / state.l[r] : 0.0f;
-                    const int64_t slot = split * all_rows + token * (to.heads * group) + head;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x[D / 16];
-#pragma unroll
-                        for (int i = 0; i < D / 16; i++) {
-                            x[i] = state.o[r][i][e] * per_sum;
-                        }
-                        const int d = g * (D / 4) + e * (D / 16);
-                        if (splits == 1) {
-                            detail::store_halves<T>(to.out + token * to.out_pitch + head * (D / 2), d, x);
-                        } else {
-                            detail::store_floats(to.partial + slot * D + d, x);
-                        }
-                    }
-                    if (splits > 1 && g == 0) {
-                        to.stats[2 * slot] = state.m[r];
-                        to.stats[2 * slot + 1] = state.l[r];
-                    }
+                for (int i = 0; i < kPart; i++) {
+                    x[i] *= per_sum;
+                }
+                detail::store_halves<T>(to.out + request.token(row) * to.out_pitch + request.head(row, piece) * (D / 2), d, x);
+            } else {
+                const int64_t part = request.part(row, piece);
+                detail::store_floats(to.partial + part * D + d, x);
+                if (d == 0) {
+                    to.stats[2 * part] = m;
+                    to.stats[2 * part + 1] = sum;
                 }
             }
         }
     }
 }
 
-// Rows of the result from the splits' parts, in the order of the splits (at most
-// 64): one wavefront a row, lane s first holds the statistics of split s.
+// One piece for MANY rows: 16 R for each of WAVES wavefronts, all against the same
+// keys.  Blocks of 16 WAVES keys are staged in LDS as the fragments that the matrix
+// instructions take, a 16-key tile by each wavefront: codes are converted and
+// values transposed once for the whole workgroup, and fragments are read 16 bytes
+// a lane without bank conflicts.  The next block's codes are loaded while this one
+// is multiplied; two buffers, one barrier a block.  Bound by the vector ALU: per
+// 16 rows and 32 keys a softmax of 8 scores a lane (8 exponentials at a quarter of
+// the rate) stands against D / 8 matrix instructions.
+template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, class T>
+__device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
+    constexpr int kRows = 16 * R, kTileRows = kRows * WAVES, kBlock = 16 * WAVES;
+    const AttentionOut &to = piece.to;
+    const int lane = lane_id(), g = lane / 16, c = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const detail::AttentionRequest<D, PAGE, T> request(batch, cache, piece);
+    const detail::KeyWalk<D, PAGE> walk = {cache, batch.table + piece.request * batch.width, piece.head, (int)batch.width, request.length, detail::opaque_zero()};
+    const int tiles = (int)to.pieces / request.splits;
+    const float scale = __builtin_fabsf(batch.scale);
+
+    __shared__ __attribute__((aligned(16))) uint32_t k_frags[2][WAVES][D / 32][kWaveSize][4];
+    __shared__ __attribute__((aligned(16))) uint32_t v_frags[2][WAVES / 2][D / 16][kWaveSize][4];
+    __shared__ __attribute__((aligned(16))) float tile_scales[2][WAVES][4];  // k, up, per_v, there
+
+    for (int tile = (int)piece.x / request.splits; tile * kTileRows < request.rows; tile += tiles) {
+        const int row0 = tile * kTileRows + wave * kRows;
+        detail::RowState<D, R, T::kBf16> state;
+        state.clear();
+        detail::load_queries(state, request, batch, piece, row0);
+        // keys that any row of the workgroup, and any / every row of this wavefront sees
+        const int all = request.limit(min((tile + 1) * kTileRows, request.rows) - 1);
+        const int most = row0 < request.rows ? request.limit(min(row0 + kRows, request.rows) - 1) : 0;
+        const int least = row0 < request.rows ? request.limit(row0) : 0;
+        const int64_t begin64 = (int64_t)request.split * to.chunk;
+        const int begin = (int)min(begin64, (int64_t)all);
+        const int end = request.split + 1 < request.splits ? (int)min(begin64 + to.chunk, (int64_t)all) : all;
+        bool missing = false;
+
+        detail::RawKeys<D> keys;
+        auto stage = [&](int buffer, int base) {
+            if (!keys.there || base + 16 > request.length) {
+                keys.clear_values_behind(base, request.length);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                const detail::Frag k = keys.template key_frag<T::kBf16>(i);
+                *reinterpret_cast<Words4 *>(k_frags[buffer][wave][i][lane]) = Words4{{k.w[0], k.w[1], k.w[2], k.w[3]}};
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                *reinterpret_cast<Words2 *>(&v_frags[buffer][wave / 2][i][lane][2 * (wave % 2)]) = keys.value_half(i);
+            }
+            const detail::TileScales scales = detail::scales_of(keys, scale);
+            if (lane == 0) {
+                const float x[4] = {scales.k, scales.up, scales.per_v, scales.there ? 1.0f : 0.0f};
+                detail::store_floats(tile_scales[buffer][wave], x);
+            }
+            missing = missing || (!keys.there && base < end);
+        };
+
+        __syncthreads();  // the previous rows' last block has been read
+        int base = begin;
+        int id = walk.look_up(base + 16 * wave);
+        if (base < end) {
+            walk.load_keys(keys, base + 16 * wave, id);
+            id = walk.look_up(base + kBlock + 16 * wave);
+            walk.load_values(keys, base + 16 * wave);
+            stage(0, base + 16 * wave);
+        }
+        __syncthreads();
+        for (int buffer = 0; base < end; buffer ^= 1) {
+            const bool more = base + kBlock < end;
+            if (more) {
+                walk.load_keys(keys, base + kBlock + 16 * wave, id);
+                id = walk.look_up(base + 2 * kBlock + 16 * wave);
+                walk.load_values(keys, base + kBlock + 16 * wave);
+            }
+#pragma unroll
+            for (int pair = 0; pair < WAVES / 2; pair++) {
+                const int at = base + 32 * pair;
+                if (at < min(most, end)) {
+                    detail::TileScales scales[2];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        uint32_t x[4];
+                        detail::load_words<4>(x, reinterpret_cast<const uint32_t *>(tile_scales[buffer][2 * pair + t]));
+                        scales[t] = {as_float((int)x[0]), as_float((int)x[1]), as_float((int)x[2]), __builtin_amdgcn_readfirstlane((int)x[3]) != 0};
+                    }
+                    const bool whole = at + 32 <= least && scales[0].there && scales[1].there;
+                    state.add(
+                        at, whole,
+                        [&](int t, int i) {
+                            detail::Frag k;
+                            detail::load_words<4>(k.w, k_frags[buffer][2 * pair + t][i][lane]);
+                            return k;
+                        },
+                        [&](int t) { return scales[t]; }, [] {},
+                        [&](int i) {
+                            detail::Frag v;
+                            detail::load_words<4>(v.w, v_frags[buffer][pair][i][lane]);
+                            return v;
+                        });
+                }
+            }
+            if (more) {
+                stage(buffer ^ 1, base + kBlock + 16 * wave);
+            }
+            __syncthreads();
+            base += kBlock;
+        }
+        if (missing && lane == 0) {
+            atomicAdd(cache.faults, 1u);
+        }
+
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float sum = detail::sum_over_lane_groups(state.l[r]);
+            const int row = row0 + 16 * r + c;
+            if (row < request.rows) {
+                const float per_sum = request.splits > 1 ? 1.0f : sum != 0.0f ? 1.0f / sum : 0.0f;
+                const int64_t part = request.part(row, piece);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x[D / 16];
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        x[i] = state.o[r][i][e] * per_sum;
+                    }
+                    const int d = g * (D / 4) + e * (D / 16);
+                    if (request.splits == 1) {
+                        detail::store_halves<T>(to.out + request.token(row) * to.out_pitch + request.head(row, piece) * (D / 2), d, x);
+                    } else {
+                        detail::store_floats(to.partial + part * D + d, x);
+                    }
+                }
+                if (request.splits > 1 && g == 0) {
+                    to.stats[2 * part] = state.m[r];
+                    to.stats[2 * part + 1] = sum;
+                }
+            }
+        }
+    }
+}
+
+// Rows of the result from the splits' parts: one workgroup a row, whose
+// wavefronts take the splits (at most 256) in turn and meet in LDS, always in the
+// same order.  A lane first holds the statistics of splits lane, lane + 64 ...
+constexpr int kSplitsPerLane = 4;
 struct JoinRows {
     uint32_t *out;
     int64_t out_pitch;
     const float *partial, *stats;
     const int32_t *starts;
-    int64_t splits, requests, q_heads, rows;
-    int64_t blocks;  // workgroups
+    int64_t splits, requests, q_heads;
+    int64_t rows;  // tokens * query heads: workgroups
 
     __device__ __forceinline__ struct JoinBlock block(int64_t x) const;
 };
@@ -541,47 +709,73 @@ template<int64_t D, int64_t WAVES, class T>
 __device__ __forceinline__ void join_splits(const AttentionBatchOf<T> &, const JoinBlock &block) {
     constexpr int kPart = D / 64;  // values a lane
     const JoinRows &to = block.to;
-    const int lane = lane_id();
-    const int64_t row = block.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    const int64_t token = row / to.q_heads;
-    if (row >= to.rows || token < to.starts[0] || token >= to.starts[to.requests]) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const int64_t row = block.x, token = row / to.q_heads;
+    if (token < to.starts[0] || token >= to.starts[to.requests]) {
         return;
     }
-    float m = detail::kLowest, l = 0.0f;
-    if (lane < to.splits) {
-        m = to.stats[2 * (lane * to.rows + row)];
-        l = to.stats[2 * (lane * to.rows + row) + 1];
+    const int splits = (int)to.splits;
+    float m[kSplitsPerLane], l[kSplitsPerLane], top = detail::kLowest;
+#pragma unroll
+    for (int j = 0; j < kSplitsPerLane; j++) {
+        const int s = j * kWaveSize + lane;
+        m[j] = detail::kLowest, l[j] = 0.0f;
+        if (s < splits) {
+            m[j] = to.stats[2 * (s * to.rows + row)];
+            l[j] = to.stats[2 * (s * to.rows + row) + 1];
+        }
+        top = __builtin_fmaxf(top, m[j]);
     }
-    float top = m;
     for (int d = 1; d < kWaveSize; d *= 2) {
         top = __builtin_fmaxf(top, __shfl_xor(top, d));
     }
-    const float weight = l != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-    float sum = l * weight;
+    __shared__ float weights[kSplitsPerLane * kWaveSize];
+    float sum = 0.0f;
+    int used = 0;  // splits up to the last one that saw any of the row's keys
+#pragma unroll
+    for (int j = 0; j < kSplitsPerLane; j++) {
+        const float weight = l[j] != 0.0f ? __builtin_amdgcn_exp2f(m[j] - top) : 0.0f;
+        sum = __builtin_fmaf(l[j], weight, sum);
+        weights[j * kWaveSize + lane] = weight;  // every wavefront writes the same
+        const uint64_t some = __ballot(l[j] != 0.0f);
+        used = some != 0 ? j * kWaveSize + 64 - __builtin_clzll(some) : used;
+    }
     for (int d = 1; d < kWaveSize; d *= 2) {
         sum += __shfl_xor(sum, d);
     }
+    __syncthreads();
     float x[kPart];
 #pragma unroll
     for (int i = 0; i < kPart; i++) {
         x[i] = 0.0f;
     }
-    for (int s = 0; s < to.splits; s++) {
-        const float w = as_float(__builtin_amdgcn_readlane(as_int(weight), s));
-        // a split that saw none of the row's keys left its part unwritten or zero
-        if (w != 0.0f) {
-            const float *part = to.partial + (s * to.rows + row) * D + lane * kPart;
+    const float *part = to.partial + row * D + lane * kPart;
+#pragma unroll 8
+    for (int s = wave; s < used; s += WAVES) {
+        const float w = weights[s];
 #pragma unroll
-            for (int i = 0; i < kPart; i++) {
-                x[i] = __builtin_fmaf(part[i], w, x[i]);
-            }
+        for (int i = 0; i < kPart; i++) {
+            // a split without any of the row's keys wrote no part
+            const float p = part[s * to.rows * D + i];
+            x[i] = __builtin_fmaf(w != 0.0f ? p : 0.0f, w, x[i]);
         }
     }
-    const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
-    unsigned short *out = reinterpret_cast<unsigned short *>(to.out + token * to.out_pitch + (row % to.q_heads) * (D / 2)) + lane * kPart;
+    __shared__ float parts[WAVES][D];
 #pragma unroll
     for (int i = 0; i < kPart; i++) {
-        out[i] = (unsigned short)(pack_halves<T>(x[i] * per_sum, 0.0f) & 0xffffu);
+        parts[wave][lane * kPart + i] = x[i];
+    }
+    __syncthreads();
+    const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
+    uint32_t *out = to.out + token * to.out_pitch + (row % to.q_heads) * (D / 2);
+    if (threadIdx.x < D / 2) {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            a += parts[w][2 * threadIdx.x];
+            b += parts[w][2 * threadIdx.x + 1];
+        }
+        out[threadIdx.x] = pack_halves<T>(a * per_sum, b * per_sum);
     }
 }
 
