@@ -319,59 +319,55 @@ def _expect(ok, what):
 
 
 class _ServingPipeline(_Pipeline):
-    """A pipeline of torch tensors: it checks types, layouts and devices before it hands addresses to the C ABI."""
+    """A pipeline of torch tensors: it checks types, layouts and devices before it hands addresses to the C ABI.  The
+    checks are written out for what they cost: a decoding step makes several of these calls of a few microseconds."""
 
-    def __init__(self):
+    def __init__(self, dtype=None):
         super().__init__()
         import torch
-        self._torch = torch
-        self._int32_type = torch.int32
         self._device = torch.cuda.current_device() if torch.cuda.is_available() else None
+        self._int32_type, self._uint8, self._float32 = torch.int32, torch.uint8, torch.float32
+        self._code_types = (torch.float8_e4m3fn, torch.uint8)
+        self._half = {"bf16": torch.bfloat16, "f16": torch.float16, None: None}[dtype]
 
     def _on_gpu(self, *tensors):
-        """All on the GPU that the pipeline was created on, which is the current one (a kernel runs where its code was loaded)."""
+        """All on the GPU that the pipeline was created on (a kernel runs where its code was loaded)."""
+        device = self._device
         for t in tensors:
-            if not t.is_cuda or t.get_device() != self._device:
-                raise GernError("every tensor must be on the pipeline's GPU (%s), not on %s" % (self._device, t.device))
-        if self._torch.cuda.current_device() != self._device:
-            raise GernError("the pipeline's GPU (%s) must be the current one" % self._device)
+            if t.get_device() != device:
+                raise GernError("every tensor must be on the pipeline's GPU (%s), not on %s" % (device, t.device))
 
     def _int32(self, **tensors):
         for name, t in tensors.items():
             if t.dtype is not self._int32_type or not t.is_contiguous():
                 raise GernError(name + " must be a contiguous int32 tensor")
 
-    def _halves(self, **tensors):
-        """16-bit floats of the pipeline's type, contiguous but for the stride of their first dimension."""
-        want = self._torch.bfloat16 if self.dtype == "bf16" else self._torch.float16
-        for name, t in tensors.items():
-            if t.dtype is not want:
-                raise GernError("%s must be %s" % (name, self.dtype))
-            inner = 1
-            for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-                if stride != inner and size != 1:
-                    raise GernError(name + " must be contiguous in all but its first dimension")
-                inner *= size
+    def _rows(self, name, t):
+        """16-bit floats of the pipeline's type, contiguous but for the stride of their first dimension, which is returned."""
+        if t.dtype is not self._half:
+            raise GernError("%s must be %s" % (name, self._half))
+        strides, shape = t.stride(), t.shape
+        inner = 1
+        for i in range(len(shape) - 1, 0, -1):
+            if strides[i] != inner and shape[i] != 1:
+                raise GernError(name + " must be contiguous in all but its first dimension")
+            inner *= shape[i]
+        return strides[0] if len(shape) > 0 and shape[0] > 1 else inner
 
     def _cache(self, k_cache, v_cache, k_scales, v_scales):
         """(pages, heads) of a paged cache."""
-        torch, shape = self._torch, k_cache.shape
+        shape = k_cache.shape
         if len(shape) != 4 or shape[2] != self.page_size or shape[3] != self.head_dim or v_cache.shape != shape:
             raise GernError("the cache's codes must be [pages, heads, page_size = %d, head_dim = %d]" % (self.page_size, self.head_dim))
         if k_scales.shape != shape[:2] or v_scales.shape != shape[:2]:
             raise GernError("the cache's scales must be [pages, heads]")
-        for t in (k_cache, v_cache):
-            if t.dtype not in (torch.float8_e4m3fn, torch.uint8) or not t.is_contiguous():
-                raise GernError("the cache's codes must be contiguous float8_e4m3fn (or uint8)")
-        for t in (k_scales, v_scales):
-            if t.dtype is not torch.float32 or not t.is_contiguous():
-                raise GernError("the cache's scales must be contiguous float32")
+        if (k_cache.dtype not in self._code_types or v_cache.dtype not in self._code_types or not k_cache.is_contiguous() or
+                not v_cache.is_contiguous()):
+            raise GernError("the cache's codes must be contiguous float8_e4m3fn (or uint8)")
+        if (k_scales.dtype is not self._float32 or v_scales.dtype is not self._float32 or not k_scales.is_contiguous() or
+                not v_scales.is_contiguous()):
+            raise GernError("the cache's scales must be contiguous float32")
         return shape[0], shape[1]
-
-
-def _pitch(t):
-    """Elements from one entry of the first dimension to the next."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t[0].numel() if t.shape[0] else 0)
 
 
 class PageTable(_ServingPipeline):
@@ -379,7 +375,7 @@ class PageTable(_ServingPipeline):
 
     def __init__(self, page_size=16, flags=0):
         super().__init__()
-        self.page_size = page_size
+        self.page_size, self._run = page_size, pipelines_lib().gern_page_table_run
         _check(pipelines_lib().gern_page_table_create(page_size, flags, C.byref(self.h)))
 
     def __call__(self, cached, added, free_pages, free_count, table, lengths, starts, slots, counts, stream=None):
@@ -387,14 +383,15 @@ class PageTable(_ServingPipeline):
         lengths [requests], starts [requests + 1], slots [tokens], counts [2] (pages left, pages missing) out; int32."""
         self._int32(cached=cached, added=added, free_pages=free_pages, free_count=free_count, table=table, lengths=lengths, starts=starts, slots=slots,
                     counts=counts)
-        n = cached.shape[0]
-        _expect(tuple(cached.shape) == tuple(added.shape) == tuple(lengths.shape) == (n,) and tuple(starts.shape) == (n + 1,) and table.dim() == 2 and
-                table.shape[0] == n and free_pages.dim() == slots.dim() == 1 and free_count.numel() == 1 and counts.numel() == 2,
-                "cached, added and lengths must be [requests], starts [requests + 1], table [requests, width], free_count [1] and counts [2]")
+        n = cached.shape[0] if cached.dim() == 1 else -1
+        _expect(n >= 0 and added.shape == lengths.shape == (n,) and starts.shape == (n + 1,) and table.dim() == 2 and table.shape[0] == n and
+                free_pages.dim() == slots.dim() == 1 and free_count.numel() == 1 and counts.numel() == 2,
+                "cached, added and lengths must be [requests], starts [requests + 1], table [requests, width], free_pages and slots one-dimensional, "
+                "free_count [1] and counts [2]")
         self._on_gpu(cached, added, free_pages, free_count, table, lengths, starts, slots, counts)
-        _check(pipelines_lib().gern_page_table_run(self.h, _ptr(cached), _ptr(added), n, _ptr(free_pages), free_pages.shape[0], _ptr(free_count),
-                                                   _ptr(table), table.shape[1], _ptr(lengths), _ptr(starts), _ptr(slots), slots.shape[0], _ptr(counts),
-                                                   stream))
+        _check(self._run(self.h, cached.data_ptr(), added.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+                         table.data_ptr(), table.shape[1], lengths.data_ptr(), starts.data_ptr(), slots.data_ptr(), slots.shape[0], counts.data_ptr(),
+                         stream))
         return table, slots
 
 
@@ -402,30 +399,31 @@ class CacheWrite(_ServingPipeline):
     """New keys and values into a paged cache in 8 bits (gern_cache_write_run)."""
 
     def __init__(self, head_dim=128, page_size=16, dtype="bf16", flags=0):
-        super().__init__()
-        self.head_dim, self.page_size, self.dtype = head_dim, page_size, dtype
-        _check(pipelines_lib().gern_cache_write_create(head_dim, page_size, _type(dtype), flags, C.byref(self.h)))
+        kind = _type(dtype)
+        super().__init__(dtype)
+        self.head_dim, self.page_size, self.dtype, self._run = head_dim, page_size, dtype, pipelines_lib().gern_cache_write_run
+        _check(pipelines_lib().gern_cache_write_create(head_dim, page_size, kind, flags, C.byref(self.h)))
 
     def __call__(self, k, v, slots, k_cache, v_cache, k_scales, v_scales, stream=None):
         """k, v [tokens, heads, head_dim] (any stride from token to token); slots [tokens] int32, -1 = not stored; the
         cache [pages, heads, page_size, head_dim] float8_e4m3fn with scales [pages, heads] float32 is updated."""
         pages, heads = self._cache(k_cache, v_cache, k_scales, v_scales)
-        n = slots.shape[0]
         self._int32(slots=slots)
-        self._halves(k=k, v=v)
-        _expect(tuple(k.shape) == tuple(v.shape) == (n, heads, self.head_dim), "k and v must be [tokens, heads, head_dim]")
+        ldk, ldv = self._rows("k", k), self._rows("v", v)
+        _expect(slots.dim() == 1 and k.shape == v.shape == (slots.shape[0], heads, self.head_dim), "slots must be [tokens], k and v [tokens, heads, head_dim]")
         self._on_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
-        _check(pipelines_lib().gern_cache_write_run(self.h, _ptr(k), _pitch(k), _ptr(v), _pitch(v), _ptr(slots), n, heads, _ptr(k_cache), _ptr(v_cache),
-                                                    _ptr(k_scales), _ptr(v_scales), pages, stream))
+        _check(self._run(self.h, k.data_ptr(), ldk, v.data_ptr(), ldv, slots.data_ptr(), slots.shape[0], heads, k_cache.data_ptr(), v_cache.data_ptr(),
+                         k_scales.data_ptr(), v_scales.data_ptr(), pages, stream))
 
 
 class CacheAttention(_ServingPipeline):
     """Causal attention of ragged batches of queries over a paged cache in 8 bits (gern_cache_attention_run)."""
 
     def __init__(self, head_dim=128, page_size=16, dtype="bf16", flags=0):
-        super().__init__()
-        self.head_dim, self.page_size, self.dtype = head_dim, page_size, dtype
-        _check(pipelines_lib().gern_cache_attention_create(head_dim, page_size, _type(dtype), flags, C.byref(self.h)))
+        kind = _type(dtype)
+        super().__init__(dtype)
+        self.head_dim, self.page_size, self.dtype, self._run = head_dim, page_size, dtype, pipelines_lib().gern_cache_attention_run
+        _check(pipelines_lib().gern_cache_attention_create(head_dim, page_size, kind, flags, C.byref(self.h)))
 
     def workspace_bytes(self, tokens, requests, q_heads, kv_heads, max_queries, max_length):
         """Bytes of device memory that a call of these sizes needs."""
@@ -440,21 +438,20 @@ class CacheAttention(_ServingPipeline):
         default what the table has room for; workspace: a uint8 tensor of workspace_bytes."""
         pages, heads = self._cache(k_cache, v_cache, k_scales, v_scales)
         self._int32(table=table, lengths=lengths, starts=starts)
-        self._halves(q=q, out=out)
-        n = lengths.shape[0]
-        _expect(q.dim() == 3 and q.shape[2] == self.head_dim and out.shape == q.shape, "q and out must be [tokens, q_heads, head_dim]")
-        _expect(table.dim() == 2 and table.shape[0] == n and tuple(lengths.shape) == (n,) and tuple(starts.shape) == (n + 1,),
+        ldq, ldo = self._rows("q", q), self._rows("out", out)
+        shape, width = q.shape, table.shape
+        _expect(len(shape) == 3 and shape[2] == self.head_dim and out.shape == shape, "q and out must be [tokens, q_heads, head_dim]")
+        _expect(len(width) == 2 and lengths.shape == (width[0],) and starts.shape == (width[0] + 1,),
                 "table must be [requests, width], lengths [requests] and starts [requests + 1]")
         self._on_gpu(q, k_cache, v_cache, k_scales, v_scales, table, lengths, starts, out)
-        ws, ws_bytes = None, 0
+        at, size = None, 0
         if workspace is not None:
             _expect(workspace.is_contiguous(), "the workspace must be contiguous")
             self._on_gpu(workspace)
-            ws, ws_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
-        _check(pipelines_lib().gern_cache_attention_run(
-            self.h, _ptr(q), _pitch(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales), pages, _ptr(table), table.shape[1], _ptr(lengths),
-            _ptr(starts), n, q.shape[0], q.shape[1], heads, _ptr(out), _pitch(out), float(scale), max_queries,
-            table.shape[1] * self.page_size if max_length is None else max_length, ws, ws_bytes, stream))
+            at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(self._run(self.h, q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, table.data_ptr(),
+                         width[1], lengths.data_ptr(), starts.data_ptr(), width[0], shape[0], shape[1], heads, out.data_ptr(), ldo, scale, max_queries,
+                         width[1] * self.page_size if max_length is None else max_length, at, size, stream))
         return out
 
 
@@ -462,23 +459,25 @@ class Matvec4(_ServingPipeline):
     """y = x W^T for up to 64 rows of x and W in 4 bits with scales (and zero points) of groups of columns (gern_matvec4_run)."""
 
     def __init__(self, group=128, dtype="bf16", flags=0):
-        super().__init__()
-        self.group, self.dtype = group, dtype
-        _check(pipelines_lib().gern_matvec4_create(group, _type(dtype), flags, C.byref(self.h)))
+        kind = _type(dtype)
+        super().__init__(dtype)
+        self.group, self.dtype, self._run = group, dtype, pipelines_lib().gern_matvec4_run
+        _check(pipelines_lib().gern_matvec4_create(group, kind, flags, C.byref(self.h)))
 
     def __call__(self, x, codes, scales, y, zeros=None, stream=None):
         """x [rows, K] and y [rows, N] (any stride from row to row); codes [N, K / 2] uint8, the even column in the lower
         half; scales [K / group, N] of x's type; zeros [K / group, N] uint8, by default 8 everywhere."""
-        uint8 = self._torch.uint8
-        self._halves(x=x, scales=scales, y=y)
-        _expect(x.dim() == y.dim() == codes.dim() == scales.dim() == 2 and y.shape[0] == x.shape[0], "x must be [rows, K], y [rows, N], codes [N, K / 2]")
+        ldx, ldy = self._rows("x", x), self._rows("y", y)
+        _expect(x.dim() == y.dim() == 2 and y.shape[0] == x.shape[0], "x must be [rows, K] and y [rows, N]")
         (m, k), n = x.shape, y.shape[1]
-        _expect(codes.dtype is uint8 and codes.is_contiguous() and codes.shape == (n, k // 2), "codes must be a contiguous uint8 tensor [N, K / 2]")
-        _expect(scales.is_contiguous() and scales.shape == (k // self.group, n), "scales must be contiguous, [K / group, N]")
-        self._on_gpu(x, codes, scales, y)
+        groups = (k // self.group, n)
+        _expect(codes.dtype is self._uint8 and codes.shape == (n, k // 2) and codes.is_contiguous(), "codes must be a contiguous uint8 tensor [N, K / 2]")
+        _expect(scales.dtype is self._half and scales.shape == groups and scales.is_contiguous(), "scales must be a contiguous tensor [K / group, N] of x's type")
+        at = None
         if zeros is not None:
-            _expect(zeros.dtype is uint8 and zeros.is_contiguous() and zeros.shape == scales.shape, "zeros must be a contiguous uint8 tensor [K / group, N]")
+            _expect(zeros.dtype is self._uint8 and zeros.shape == groups and zeros.is_contiguous(), "zeros must be a contiguous uint8 tensor [K / group, N]")
             self._on_gpu(zeros)
-        _check(pipelines_lib().gern_matvec4_run(self.h, _ptr(x), _pitch(x), _ptr(codes), _ptr(scales), None if zeros is None else _ptr(zeros), _ptr(y),
-                                                _pitch(y), m, n, k, stream))
+            at = zeros.data_ptr()
+        self._on_gpu(x, codes, scales, y)
+        _check(self._run(self.h, x.data_ptr(), ldx, codes.data_ptr(), scales.data_ptr(), at, y.data_ptr(), ldy, m, n, k, stream))
         return y

@@ -688,6 +688,14 @@ int gern_hip_device_limits(gern_hip_limits *out) {
     return current_limits(*out);
 }
 
+int gern_hip_current_device(int *device) {
+    if (device == nullptr) {
+        return fail(GERN_HIP_ERR_ARGUMENT, "gern_hip_current_device: null argument");
+    }
+    HIP_TRY(hipGetDevice(device));
+    return GERN_HIP_OK;
+}
+
 int gern_hip_device_count(int *count) {
     if (count == nullptr) {
         return fail(GERN_HIP_ERR_ARGUMENT, "gern_hip_device_count: null output");

@@ -45,6 +45,7 @@ struct gern_pipeline_s {
     };
     std::vector<Variant> variants;
     size_t last_variant = 0;
+    int device = 0;  // the GPU that was current at creation, where the programs are loaded
     int64_t page_size = 0, group = 0;
     uint32_t *fault_count = nullptr;  // one device word: slots and pages outside the cache (gern_pipeline_faults)
     // parameter names

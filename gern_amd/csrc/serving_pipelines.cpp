@@ -44,6 +44,9 @@ public:
             const std::string name = one.runner ? one.runner->getKernelName() : one.kernel_name;
             p->variants.push_back({std::move(one.runner), one.source, name});
         }
+        if (rc == 0 && !compile_only && gern_hip_current_device(&p->device) != 0) {
+            return failHip("gern_hip_current_device");
+        }
         return rc;
     }
     // The device word that gern_pipeline_faults reads.
@@ -81,6 +84,14 @@ int evaluate(gern_pipeline p, size_t variant, const char *who, void *stream, con
         Runner *runner = p->variants[variant].runner.get();
         if (runner == nullptr) {
             return fail(std::string(who) + ": the pipeline was created compile-only");
+        }
+        int device = -1;
+        if (gern_hip_current_device(&device) != 0) {
+            return failHip(who);
+        }
+        if (device != p->device) {
+            return fail(std::string(who) + ": the pipeline was created on GPU " + std::to_string(p->device) + ", and GPU " + std::to_string(device) +
+                        " is current");
         }
         runner->setStream(stream);
         runner->evaluate(args);

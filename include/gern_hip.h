@@ -121,6 +121,8 @@ int gern_hip_event_destroy(gern_hip_event ev);
 /* Limits of device 0, cached after the first call. */
 int gern_hip_device_limits(gern_hip_limits *out);
 int gern_hip_device_count(int *count);
+/* The calling thread's current device. */
+int gern_hip_current_device(int *device);
 
 /* Copies the calling thread's last error message (NUL-terminated, possibly
  * truncated) into buf; returns the full length of the message. */
