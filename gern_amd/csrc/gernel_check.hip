@@ -208,7 +208,10 @@ __global__ void __launch_bounds__(512) check_matvec4(gernels::ActivationsOf<T> x
     auto columns = y.at(blockIdx.x);
     gernels::multiply_4bit<G, MT, NT, 8>(x.whole(), weights.whole(), columns);
 }
+template __global__ void check_matvec4<128, 0, 1, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<128, 0, 4, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<32, 0, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
 template __global__ void check_matvec4<128, 1, 1, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
-template __global__ void check_matvec4<128, 1, 2, gernels::Bf16>(gernels::ActivationsOf<gernels::Bf16>, gernels::Weights4, gernels::MatvecOut);
-template __global__ void check_matvec4<64, 2, 2, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
-template __global__ void check_matvec4<32, 4, 2, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<64, 1, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<64, 2, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
+template __global__ void check_matvec4<32, 4, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <iterator>
 
 using namespace gern;
 using gern_detail::fail;
@@ -529,9 +530,34 @@ namespace {
 struct MatvecShape {
     int64_t row_tiles, column_tiles;
 };
-// The programs of a pipeline; 8 wavefronts each.
-constexpr MatvecShape kMatvecShapes[] = {{1, 1}, {1, 2}, {2, 2}, {4, 2}};
+// The programs of a pipeline, by tiles of 16 rows (0: up to 4 rows) and of 16 columns; 8 wavefronts each.
+constexpr MatvecShape kMatvecShapes[] = {{0, 1}, {0, 2}, {0, 4}, {1, 1}, {1, 2}, {1, 3}, {1, 4}, {2, 1}, {2, 4}, {4, 1}, {4, 4}};
 constexpr int64_t kMatvecWaves = 8;
+
+// The program for M rows and N columns: the one whose slowest CU has least to do.  A workgroup's work is its tiles of
+// columns, and what it does for x whatever their number: as much as 0.7 of a tile with up to 4 rows, as 2 tiles for
+// every 16 rows beyond that.  Measured (us, K = 8192 but where said), one to four tiles of columns:
+//   1 row:   28672 columns 33 / 31 / 31 / 30, 16384 of K = 4096 9.7 / 9.8 / - / 9.2, 8192 11.3 / 9.7 / - / 12.5
+//   13 rows: 10001 columns 27 / 24 / 16.6 / 18.7;  16 rows: 20000 - / - / 33 / 37, 32768 of K = 4096 - / - / 25 / 21
+//   8 rows:  6000 columns 16 / 12 / 14 / -, 4096 of K = 4096 7.2 / 7.7 / 8.4 / -
+//   32 rows: 16384 columns - / 43 / - / 32, 4096 of K = 4096 11 / 13 / - / 16
+size_t matvecVariant(int64_t M, int64_t N) {
+    const int64_t row_tiles = M <= 4 ? 0 : M <= 16 ? 1 : M <= 32 ? 2 : 4, tiles = (N + 15) / 16;
+    size_t best = 0;
+    int64_t least = INT64_MAX;
+    for (size_t i = 0; i < std::size(kMatvecShapes); i++) {
+        const MatvecShape &shape = kMatvecShapes[i];
+        if (shape.row_tiles == row_tiles) {
+            const int64_t workgroups = (tiles + shape.column_tiles - 1) / shape.column_tiles, rounds = (workgroups + 255) / 256;
+            const int64_t work = rounds * (10 * shape.column_tiles + (row_tiles == 0 ? 7 : 20 * row_tiles));
+            if (work < least) {
+                least = work;
+                best = i;
+            }
+        }
+    }
+    return best;
+}
 
 }  // namespace
 
@@ -574,8 +600,9 @@ int gern_matvec4_run(gern_pipeline p, const void *X, int64_t ldx, const uint8_t 
     if (!usable(p, gern_pipeline_s::MATVEC4)) {
         return fail("gern_matvec4_run: bad pipeline");
     }
-    if (M < 0 || M > GERN_MATVEC4_MAX_ROWS || N < 1 || N > 0x7fffffff || K < 1 || K > 0x7fffffff || K % p->group != 0) {
-        return fail("gern_matvec4_run: M must be in [0, GERN_MATVEC4_MAX_ROWS = 64], N and K in [1, 2^31), and K a multiple of the group");
+    if (M < 0 || M > GERN_MATVEC4_MAX_ROWS || N < 1 || N > 0x7fffffff || K < 1 || K > GERN_MATVEC4_MAX_COLUMNS || K % p->group != 0) {
+        return fail("gern_matvec4_run: M must be in [0, GERN_MATVEC4_MAX_ROWS = 64], N in [1, 2^31), K in [1, GERN_MATVEC4_MAX_COLUMNS = 2^24] and a "
+                    "multiple of the group");
     }
     if (M == 0) {
         return 0;
@@ -587,17 +614,15 @@ int gern_matvec4_run(gern_pipeline p, const void *X, int64_t ldx, const uint8_t 
         return fail("gern_matvec4_run: X and the codes are read in 16-byte pieces: both must be 16-byte aligned and the row stride of X a multiple of 8 "
                     "elements (scales and Y 2-byte aligned)");
     }
-    if (M > 1 && (ldx < K || ldy < N)) {
-        return fail("gern_matvec4_run: a row stride is less than its row");
+    if (M > 1 && (ldx < K || ldx > 2 * GERN_MATVEC4_MAX_COLUMNS || ldy < N)) {
+        return fail("gern_matvec4_run: a row stride is less than its row, or that of X more than 2 * GERN_MATVEC4_MAX_COLUMNS");
     }
     const int64_t x_bytes = ((M - 1) * ldx + K) * 2, y_bytes = ((M - 1) * ldy + N) * 2, groups = K / p->group;
     if (overlap(Y, y_bytes, X, x_bytes) || overlap(Y, y_bytes, codes, N * K / 2) || overlap(Y, y_bytes, scales, groups * N * 2) ||
         overlap(Y, y_bytes, zeros, zeros != nullptr ? groups * N : 0)) {
         return fail("gern_matvec4_run: Y shares memory with an input");
     }
-    // Two tiles of 16 columns a workgroup, so that x is read for 32 columns at a time; one where that leaves fewer
-    // workgroups than two for each of 256 CUs.
-    const size_t variant = M > 32 ? 3 : M > 16 ? 2 : N > 16384 ? 1 : 0;
+    const size_t variant = matvecVariant(M, N);
     const int64_t tile = 16 * kMatvecShapes[variant].column_tiles;
     hip::Activations x{X, ldx / 2, M};
     hip::Weights4 weights{codes, scales, zeros, N, K};

@@ -18,10 +18,13 @@
 // sum x (128 + q) - (128 + z) sum x.  The sum of x comes from one more matrix
 // instruction, against ones, for all columns.  The offset costs fp32 rounding of a
 // sum 128 / 4.6 (the spread of q - z) times larger: 2^-24 * 28, 2^-19.2 of the
-// result's size against the 2^-9 (bf16) or 2^-12 (fp16) of its last rounding.
+// result's size against the 2^-8 (bf16) or 2^-11 (fp16) of its last rounding.
 //
 // The wavefronts of a workgroup divide K and add their sums in LDS, in a fixed
-// order.
+// order.  Measured: 1 row, 28672 columns, K = 8192, G = 128 in 27.6 us (4.5 TB/s of
+// codes, scales and zero points; a copy of 1 GiB moves 5.2 on the same GPU); 13
+// rows, 10001 columns, K = 8192, G = 64 in 15.6 us (2.9 TB/s: bound by the vector
+// ALU, which takes 7 instructions for 8 codes and 8 for the sums of a group).
 #pragma once
 
 #include "gernels/half_tiles.h"
@@ -87,14 +90,19 @@ template<bool BF16>
 struct CodeOffset {
     static constexpr float value = BF16 ? 128.0f : 64.0f;
 };
+// `offsets` is code_offsets<BF16>(): in a register, so that `and` and `or` are one instruction (two literals do not fit).
 template<bool BF16>
-__device__ __forceinline__ Frag offset_codes(uint32_t w) {
+__device__ __forceinline__ uint32_t code_offsets() {
+    uint32_t two = BF16 ? 0x43004300u : 0x54005400u;
+    asm volatile("" : "+v"(two));
+    return two;
+}
+template<bool BF16>
+__device__ __forceinline__ Frag offset_codes(uint32_t w, uint32_t offsets) {
     if constexpr (BF16) {
-        return {{(w & 0x000f000fu) | 0x43004300u, ((w >> 4) & 0x000f000fu) | 0x43004300u, ((w >> 8) & 0x000f000fu) | 0x43004300u,
-                 ((w >> 12) & 0x000f000fu) | 0x43004300u}};
+        return {{(w & 0x000f000fu) | offsets, ((w >> 4) & 0x000f000fu) | offsets, ((w >> 8) & 0x000f000fu) | offsets, ((w >> 12) & 0x000f000fu) | offsets}};
     } else {
-        return {{((w << 4) & 0x00f000f0u) | 0x54005400u, (w & 0x00f000f0u) | 0x54005400u, ((w >> 4) & 0x00f000f0u) | 0x54005400u,
-                 ((w >> 8) & 0x00f000f0u) | 0x54005400u}};
+        return {{((w << 4) & 0x00f000f0u) | offsets, (w & 0x00f000f0u) | offsets, ((w >> 4) & 0x00f000f0u) | offsets, ((w >> 8) & 0x00f000f0u) | offsets}};
     }
 }
 
@@ -104,115 +112,222 @@ __device__ __forceinline__ Frag pair_with_fourth(const Frag &x) {
              __builtin_amdgcn_perm(x.w[3], x.w[1], 0x05040100u), __builtin_amdgcn_perm(x.w[3], x.w[1], 0x07060302u)}};
 }
 
-// One block of 128 k: codes, activations, scales and zero points.
+// All four lane groups get, in register t, what lane group t has in w: the transposition of four equal registers.
+__device__ __forceinline__ void spread_lane_groups(uint32_t w, uint32_t to[4]) {
+    to[0] = to[1] = to[2] = to[3] = w;
+    transpose_lane_groups(to);
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// One block of 128 k as it is loaded: codes, activations, scales and zero points.  Vectors, not arrays: a loaded vector
+// that is carried to the next iteration as four words is copied word by word, and waited for, where it is loaded.
+// With three or four tiles of columns, lane group t holds the scales and zero points of tile t, one load for all;
+// otherwise each tile's are in every lane group.
 template<int G, int MT, int NT>
 struct MatvecBlock {
-    uint32_t codes[NT][4];
-    Frag x[MT][4];
-    uint32_t scale[NT][128 / G], zero[NT][128 / G];
+    static constexpr int kXTiles = MT == 0 ? 1 : MT, kXSteps = MT == 0 ? 1 : 4, kScaleTiles = NT >= 3 ? 1 : NT;
+    u32x4 codes[NT];
+    u32x4 x[kXTiles][kXSteps];
+    uint32_t scale[kScaleTiles][128 / G], zero[kScaleTiles][128 / G];
 };
 
 }  // namespace detail
 
-// MT tiles of 16 rows against NT tiles of 16 columns on WAVES wavefronts.
+// NT (1 to 4) tiles of 16 columns on WAVES wavefronts, for up to 16 MT rows of x; MT = 0: up to 4 rows.
+//
+// With up to 4 rows the 16 rows of a matrix instruction hold them four times over, shifted: row 4 i + s is row i at
+// step s of a block (k = 32 s ..).  One load brings x for all four steps, and step s's products stand in row 4 i + s of
+// an accumulator of its own, element s of lane group i: four times less x to load and to arrange.
 template<int64_t G, int64_t MT, int64_t NT, int64_t WAVES, class T>
 __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const Weights4 &weights, const MatvecColumns &columns) {
-    constexpr bool kBf16 = T::kBf16;
+    constexpr bool kBf16 = T::kBf16, kFew = MT == 0;
     constexpr int kGroups = 128 / G;  // of a block
     constexpr int kSteps = G / 32;    // of a group
+    constexpr int kRowTiles = kFew ? 1 : MT, kSums = kFew ? 1 : 4;  // sums a lane holds of a tile
+    using Block = detail::MatvecBlock<G, MT, NT>;
     const int lane = lane_id(), g = lane / 16, c = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const int64_t n0 = columns.x * (16 * NT);
-    const int blocks = (int)((weights.k + 127) / 128);
-    const int groups = (int)(weights.k / G);
+    const int words = (int)(weights.k / 8), blocks = (words + 15) / 16;
 
-    // rows and columns behind the last one read it again; their sums are not stored
-    const uint32_t *code_row[NT];
-    int64_t column[NT];
+    // Addresses are a uniform base, which the scalar unit advances, and a lane's offset, which stays.  Rows and columns
+    // behind the last one read it again; their sums are not stored.  A last block that is not whole is read as the
+    // LAST 128 columns (fewer, where there are not that many), and x is zero in those that an earlier block had.  No load
+    // stands behind a branch: what a branch may leave unloaded is waited for where the paths meet, and loads are to run
+    // ahead of their use.
+    const int last_column = (int)min(weights.n - 1 - n0, (int64_t)(16 * NT - 1));
+    uint32_t code_offset[NT], x_offset[kRowTiles], scale_offset[Block::kScaleTiles];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        column[t] = min(n0 + 16 * t + c, weights.n - 1);
-        code_row[t] = weights.codes + column[t] * (weights.k / 8) + 4 * g;
+        code_offset[t] = (uint32_t)min(16 * t + c, last_column) * (uint32_t)words + (uint32_t)min(4 * g, words - 4);
     }
-    auto load = [&](detail::MatvecBlock<G, MT, NT> &b, int block) {
-        // a last block may be 32, 64 or 96 wide: its missing x are zero, and its missing codes are the row's first
-        const int64_t k0 = (int64_t)block * 128;
-        const int64_t word = k0 + 32 * g < weights.k ? k0 / 8 : -4 * g;
+#pragma unroll
+    for (int t = 0; t < Block::kScaleTiles; t++) {
+        scale_offset[t] = (uint32_t)min(16 * (NT >= 3 ? g : t) + c, last_column);
+    }
+    const int last_row = (int)a.rows - 1;
+#pragma unroll
+    for (int r = 0; r < kRowTiles; r++) {
+        const int row = min(kFew ? c / 4 : 16 * r + c, last_row);
+        x_offset[r] = (uint32_t)(row * (int)a.pitch + 4 * g + (kFew ? min(16 * (c % 4), 4 * words - 16) : 0));
+    }
+    const bool with_zeros = weights.zeros != nullptr;
+    const uint32_t *codes = weights.codes + n0 * words;
+    const unsigned short *scales = weights.scales + n0;
+    const unsigned char *zeros = with_zeros ? weights.zeros + n0 : reinterpret_cast<const unsigned char *>(weights.scales);
+
+    auto load = [&](Block &b, int block) {
+        const int first = max(min(16 * block, words - 16), 0);  // in words of codes
+        const uint32_t *block_codes = codes + first;
+        const uint32_t *block_x = a.x + 4 * first;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            detail::load_words<4>(b.codes[t], code_row[t] + word);
+            b.codes[t] = *reinterpret_cast<const detail::u32x4 *>(block_codes + code_offset[t]);
+        }
 #pragma unroll
-            for (int j = 0; j < kGroups; j++) {
-                const int64_t at = min((int)(block * kGroups) + j, groups - 1) * weights.n + column[t];
-                b.scale[t][j] = weights.scales[at];
-                b.zero[t][j] = weights.zeros != nullptr ? weights.zeros[at] : 8;
+        for (int r = 0; r < kRowTiles; r++) {
+#pragma unroll
+            for (int s = 0; s < Block::kXSteps; s++) {
+                b.x[r][s] = *reinterpret_cast<const detail::u32x4 *>(block_x + (kFew ? 0 : min(16 * s, 4 * words - 16)) + x_offset[r]);
             }
         }
 #pragma unroll
-        for (int r = 0; r < MT; r++) {
+        for (int j = 0; j < kGroups; j++) {
+            // a block of fewer than 128 columns has fewer groups: the last one again
+            const int64_t group_row = (int64_t)min(first * 8 / (int)G + j, words * 8 / (int)G - 1) * weights.n;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                b.x[r][s] = detail::Frag{{0u, 0u, 0u, 0u}};
-                if (16 * r + c < a.rows && k0 + 32 * s < weights.k) {
-                    detail::load_words<4>(b.x[r][s].w, a.x + (16 * r + c) * a.pitch + (k0 + 32 * s + 8 * g) / 2);
-                }
+            for (int t = 0; t < Block::kScaleTiles; t++) {
+                b.scale[t][j] = (scales + group_row)[scale_offset[t]];
+                b.zero[t][j] = (zeros + group_row)[scale_offset[t]];
             }
         }
     };
 
-    detail::f32x4 total[NT][MT];
+    float total[NT][kRowTiles][kSums];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int r = 0; r < MT; r++) {
-            total[t][r] = detail::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < kRowTiles; r++) {
+#pragma unroll
+            for (int e = 0; e < kSums; e++) {
+                total[t][r][e] = 0.0f;
+            }
         }
     }
     constexpr uint32_t kOnes = kBf16 ? 0x3f803f80u : 0x3c003c00u;
     const detail::Frag ones = {{kOnes, kOnes, kOnes, kOnes}};
-    auto add = [&](detail::MatvecBlock<G, MT, NT> &b) {
+    const detail::f32x4 nothing = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t offsets = detail::code_offsets<kBf16>();
+    auto add = [&](Block &b, int block, bool may_be_last) {
+        if (may_be_last && 16 * block + 16 > words) {
+            // x is zero in front of this block's columns and behind the last one
+            const int first = max(min(16 * block, words - 16), 0);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            detail::transpose_lane_groups(b.codes[t]);
-        }
+            for (int r = 0; r < kRowTiles; r++) {
 #pragma unroll
-        for (int j = 0; j < kGroups; j++) {
-            detail::f32x4 dot[NT][MT], sum[MT];
-#pragma unroll
-            for (int r = 0; r < MT; r++) {
-                sum[r] = detail::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    dot[t][r] = sum[r];
+                for (int s = 0; s < Block::kXSteps; s++) {
+                    const int word = first + 4 * (kFew ? c % 4 : s);
+                    if (word < 16 * block || word >= words) {
+                        b.x[r][s] = detail::u32x4{0u, 0u, 0u, 0u};
+                    }
                 }
             }
+        }
+        detail::Frag x[kRowTiles][Block::kXSteps];
 #pragma unroll
-            for (int i = 0; i < kSteps; i++) {
-                const int s = j * kSteps + i;
-                detail::Frag x[MT];
+        for (int r = 0; r < kRowTiles; r++) {
 #pragma unroll
-                for (int r = 0; r < MT; r++) {
-                    x[r] = detail::pair_with_fourth(b.x[r][s]);
-                    sum[r] = detail::mfma_16x16x32<kBf16>(x[r], ones, sum[r]);
-                }
+            for (int s = 0; s < Block::kXSteps; s++) {
+                x[r][s] = detail::pair_with_fourth(__builtin_bit_cast(detail::Frag, b.x[r][s]));
+            }
+        }
+        uint32_t block_codes[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                block_codes[t][s] = b.codes[t][s];
+            }
+            detail::transpose_lane_groups(block_codes[t]);
+        }
+        const detail::f32x4 sum_of_steps = kFew ? detail::mfma_16x16x32<kBf16>(x[0][0], ones, nothing) : nothing;
+#pragma unroll
+        for (int j = 0; j < kGroups; j++) {
+            uint32_t scale_zero[4];  // scale in the low half, zero point above it
+            if constexpr (NT >= 3) {
+                detail::spread_lane_groups(b.scale[0][j] | b.zero[0][j] << 16, scale_zero);
+            } else {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const detail::Frag w = detail::offset_codes<kBf16>(b.codes[t][s]);
+                    scale_zero[t] = b.scale[t][j] | b.zero[t][j] << 16;
+                }
+            }
+            float sum[kRowTiles][kSums];
 #pragma unroll
-                    for (int r = 0; r < MT; r++) {
-                        dot[t][r] = detail::mfma_16x16x32<kBf16>(x[r], w, dot[t][r]);
+            for (int r = 0; r < kRowTiles; r++) {
+                if constexpr (kFew) {
+                    sum[0][0] = sum_of_steps[j * kSteps];
+#pragma unroll
+                    for (int i = 1; i < kSteps; i++) {
+                        sum[0][0] += sum_of_steps[j * kSteps + i];
+                    }
+                } else {
+                    detail::f32x4 of_group = nothing;
+#pragma unroll
+                    for (int i = 0; i < kSteps; i++) {
+                        of_group = detail::mfma_16x16x32<kBf16>(x[r][j * kSteps + i], ones, of_group);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sum[r][e] = of_group[e];
                     }
                 }
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const float scale = half_to_float<T>(b.scale[t][j]);
-                const float zero = -((float)b.zero[t][j] + detail::CodeOffset<kBf16>::value);
+                float dot[kRowTiles][kSums];
+                if constexpr (kFew) {
+                    detail::f32x4 of_step[kSteps];
 #pragma unroll
-                for (int r = 0; r < MT; r++) {
+                    for (int i = 0; i < kSteps; i++) {
+                        of_step[i] = detail::mfma_16x16x32<kBf16>(x[0][0], detail::offset_codes<kBf16>(block_codes[t][j * kSteps + i], offsets), nothing);
+                    }
+                    dot[0][0] = of_step[0][j * kSteps];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        total[t][r][e] = __builtin_fmaf(scale, __builtin_fmaf(zero, sum[r][e], dot[t][r][e]), total[t][r][e]);
+                    for (int i = 1; i < kSteps; i++) {
+                        dot[0][0] += of_step[i][j * kSteps + i];
+                    }
+                } else {
+                    detail::f32x4 of_group[kRowTiles];
+#pragma unroll
+                    for (int r = 0; r < kRowTiles; r++) {
+                        of_group[r] = nothing;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kSteps; i++) {
+                        const int s = j * kSteps + i;
+                        const detail::Frag w = detail::offset_codes<kBf16>(block_codes[t][s], offsets);
+#pragma unroll
+                        for (int r = 0; r < kRowTiles; r++) {
+                            of_group[r] = detail::mfma_16x16x32<kBf16>(x[r][s], w, of_group[r]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < kRowTiles; r++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            dot[r][e] = of_group[r][e];
+                        }
+                    }
+                }
+                const float scale = half_to_float<T>(scale_zero[t] & 0xffffu);
+                const float zero = -((with_zeros ? (float)(scale_zero[t] >> 16) : 8.0f) + detail::CodeOffset<kBf16>::value);
+#pragma unroll
+                for (int r = 0; r < kRowTiles; r++) {
+#pragma unroll
+                    for (int e = 0; e < kSums; e++) {
+                        total[t][r][e] = __builtin_fmaf(scale, __builtin_fmaf(zero, sum[r][e], dot[r][e]), total[t][r][e]);
                     }
                 }
             }
@@ -220,51 +335,61 @@ __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const W
     };
 
     int block = wave;
-    if (block < blocks) {
-        detail::MatvecBlock<G, MT, NT> even, odd;
-        load(even, block);
-        while (true) {
+    if constexpr (MT <= 1) {
+        // The next block's loads are issued in front of this one's products, and the barriers keep them there.
+        if (block < blocks) {
+            Block even, odd;
+            load(even, block);
+            for (; block + 2 * WAVES < blocks; block += 2 * WAVES) {
+                load(odd, block + WAVES);
+                __builtin_amdgcn_sched_barrier(0);
+                add(even, block, false);
+                __builtin_amdgcn_sched_barrier(0);
+                load(even, block + 2 * WAVES);
+                __builtin_amdgcn_sched_barrier(0);
+                add(odd, block + WAVES, false);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (block + WAVES < blocks) {
                 load(odd, block + WAVES);
+                __builtin_amdgcn_sched_barrier(0);
+                add(even, block, true);
+                add(odd, block + WAVES, true);
+            } else {
+                add(even, block, true);
             }
-            add(even);
-            block += WAVES;
-            if (block >= blocks) {
-                break;
-            }
-            if (block + WAVES < blocks) {
-                load(even, block + WAVES);
-            }
-            add(odd);
-            block += WAVES;
-            if (block >= blocks) {
-                break;
-            }
+        }
+    } else {
+        // two blocks of x do not fit beside the sums
+        for (; block < blocks; block += WAVES) {
+            Block b;
+            load(b, block);
+            add(b, block, true);
         }
     }
 
-    // [wavefront][tile][row of four][lane]
-    constexpr int kTiles = NT * MT;
-    __shared__ float parts[WAVES][kTiles * 4][kWaveSize];
+    // [wavefront][tile and sum][lane]
+    constexpr int kParts = NT * kRowTiles * kSums;
+    __shared__ float parts[WAVES][kParts][kWaveSize];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int r = 0; r < MT; r++) {
+        for (int r = 0; r < kRowTiles; r++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                parts[wave][(t * MT + r) * 4 + e][lane] = total[t][r][e];
+            for (int e = 0; e < kSums; e++) {
+                parts[wave][(t * kRowTiles + r) * kSums + e][lane] = total[t][r][e];
             }
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < kTiles * 4 * kWaveSize; i += WAVES * kWaveSize) {
+    for (int i = threadIdx.x; i < kParts * kWaveSize; i += WAVES * kWaveSize) {
         float y = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
             y += parts[w][i / kWaveSize][i % kWaveSize];
         }
-        const int from = i % kWaveSize, tile = i / kWaveSize / 4, e = i / kWaveSize % 4;
-        const int64_t m = 16 * (tile % MT) + 4 * (from / 16) + e, n = n0 + 16 * (tile / MT) + from % 16;
+        const int from = i % kWaveSize, tile = i / kWaveSize / kSums, e = i / kWaveSize % kSums;
+        const int64_t m = kFew ? from / 16 : 16 * (tile % kRowTiles) + 4 * (from / 16) + e, n = n0 + 16 * (tile / kRowTiles) + from % 16;
         if (m < a.rows && n < weights.n) {
             columns.to.y[m * columns.to.pitch + n] = (unsigned short)(pack_halves<T>(y, 0.0f) & 0xffffu);
         }
