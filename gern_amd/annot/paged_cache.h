@@ -55,7 +55,7 @@ struct JoinRows {
     int64_t out_pitch;
     const float *partial, *stats;
     const int32_t *starts;
-    int64_t splits, requests, q_heads, rows;
+    int64_t splits, requests, q_heads, rows, blocks;
 };
 
 }  // namespace hip

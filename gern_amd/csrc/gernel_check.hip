@@ -189,17 +189,18 @@ template __global__ void check_attend_few<128, 64, gernels::Bf16>(gernels::Atten
 template __global__ void check_attend_few<128, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
 template __global__ void check_attend_few<192, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
 template __global__ void check_attend_few<256, 16, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
-template __global__ void check_attend_many<64, 32, 4, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
+template __global__ void check_attend_many<64, 32, 2, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
 template __global__ void check_attend_many<128, 16, 2, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
 template __global__ void check_attend_many<192, 64, 1, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::PagedCache, gernels::AttentionOut);
 template __global__ void check_attend_many<256, 16, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::PagedCache, gernels::AttentionOut);
 
-template<int64_t D, class T>
+template<int64_t D, int64_t PER_ROW, class T>
 __global__ void __launch_bounds__(256) check_join_splits(gernels::AttentionBatchOf<T> batch, gernels::JoinRows rows) {
     auto block = rows.block(blockIdx.x);
-    gernels::join_splits<D, 4>(batch.whole(), block);
+    gernels::join_splits<D, 4, PER_ROW>(batch.whole(), block);
 }
-template __global__ void check_join_splits<192, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::JoinRows);
+template __global__ void check_join_splits<192, 4, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::JoinRows);
+template __global__ void check_join_splits<64, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::JoinRows);
 
 #include "gernels/matvec4.h"
 

@@ -352,7 +352,9 @@ int attentionResidentWaves(int64_t head_dim) {
 
 AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, int64_t rows, int64_t max_length) {
     AttentionPlan plan{};
-    plan.variant = rows <= 32 ? 0 : 1;
+    // 32 requests of 2000 to 4000 keys, 8 heads of 128, us with few / many rows a program: 16 rows 56 / 91, 32 rows 63 / 93,
+    // 64 rows 91 / 101.
+    plan.variant = rows <= 64 ? 0 : 1;
     const int64_t tile = plan.variant == 0 ? 16 : 16 * kAttentionWaves * attentionRowTiles(head_dim);
     plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
     // Keys are split, into pieces of at least 256, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
@@ -360,7 +362,7 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     // more than 128 dimensions: two, what is resident, because the joined parts are larger and a start costs more.
     // Measured (us) with 512 / 1024 / 2048 / 4096: 64 requests of 4096 to 8192 keys, 8 heads of 128: 181 / 175 / 155 /
     // 165; 3 of 131072 to 262144: 266 / 188 / 184 / 197; 32 of 1250 to 2500, 16 heads of 256: 95 / 110 / 109 / -; 6 of 113
-    // to 447 queries and 4032 to 5915 keys, 4 heads of 64 for 16: 166 / 124 / 116 / -.
+    // to 447 queries and 4032 to 5915 keys, 4 heads of 64 for 16: - / 103 / 97 / 103.
     const int64_t wanted = plan.variant == 0 && head_dim > 128 ? 512 : 2048;
     const int64_t whole = requests * heads * plan.row_tiles;
     const int64_t splits = std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
@@ -429,19 +431,24 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
                 (Tile(result["pieces"], x.bind(1)) || Grid::BLOCK_Y)((Tile(result["heads"], head.bind(1)) || Grid::BLOCK_X)(
                     (Tile(result["requests"], request.bind(1)) || Grid::BLOCK_Z)(attend[bound](batch, cache, result)))),
                 {{Grid::BLOCK_DIM_X, threads.bind(64 * kAttentionWaves)}});
-            // two wavefronts of the second program on a SIMD, where its staged keys leave room in LDS
-            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP, few ? attentionResidentWaves(head_dim) : head_dim <= 128 ? 2 : 1) != 0) {
+            // wavefronts of the second program on a SIMD
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP, few ? attentionResidentWaves(head_dim) : head_dim == 64 ? 3 : 2) != 0) {
                 return 1;
             }
         }
         using Rows = hip::JoinRows;
-        AbstractDataTypePtr rows(new const annot::PiecesADT<Rows>("rows", "gernels::JoinRows", "block", {{"rows", &Rows::rows}}));
-        annot::PieceFunction join("gernels::join_splits", header, {batch}, rows, {"rows"}, {"head_dim", "waves"});
-        Variable x("x"), threads("threads");
-        Composable program = Global((Tile(rows["rows"], x.bind(1)) || Grid::BLOCK_X)(
-                                        join[{constant("head_dim", head_dim), constant("waves", 4)}](batch, rows)),
-                                    {{Grid::BLOCK_DIM_X, threads.bind(256)}});
-        if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0 || p.addFaultCount("gern_cache_attention_create") != 0) {
+        for (int64_t per_row : {1, 4}) {
+            AbstractDataTypePtr rows(new const annot::PiecesADT<Rows>("rows", "gernels::JoinRows", "block", {{"blocks", &Rows::blocks}}));
+            annot::PieceFunction join("gernels::join_splits", header, {batch}, rows, {"blocks"}, {"head_dim", "waves", "per_row"});
+            Variable x("x"), threads("threads");
+            Composable program = Global((Tile(rows["blocks"], x.bind(1)) || Grid::BLOCK_X)(
+                                            join[{constant("head_dim", head_dim), constant("waves", 4), constant("per_row", per_row)}](batch, rows)),
+                                        {{Grid::BLOCK_DIM_X, threads.bind(256)}});
+            if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP) != 0) {
+                return 1;
+            }
+        }
+        if (p.addFaultCount("gern_cache_attention_create") != 0) {
             return 1;
         }
         *out = p.handOut();
@@ -517,8 +524,9 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     if (rc != 0 || plan.splits == 1) {
         return rc;
     }
-    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows};
-    const int joined = evaluate(p, 2, who, stream, {{"batch", &batch}, {"rows", &join}});
+    const bool wave_a_row = plan.splits <= 16;
+    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, wave_a_row ? (rows + 3) / 4 : rows};
+    const int joined = evaluate(p, wave_a_row ? 2 : 3, who, stream, {{"batch", &batch}, {"rows", &join}});
     p->last_variant = plan.variant;
     return joined;
 }

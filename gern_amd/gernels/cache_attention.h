@@ -94,6 +94,14 @@ __device__ __forceinline__ uint32_t codes_to_halves(uint32_t w) {
     }
 }
 
+// The larger of two numbers that are not NaN.  fmaxf first quiets operands that it does not know to be results of
+// arithmetic (products of the matrix cores, lanes exchanged), an instruction each; the median with infinity does not.
+__device__ __forceinline__ float larger(float a, float b) {
+    float infinity = __builtin_inff();
+    asm("" : "+s"(infinity));  // or the compiler makes it fmaxf again
+    return __builtin_amdgcn_fmed3f(a, b, infinity);
+}
+
 // Maximum / sum over the four lanes with the same lane mod 16.
 template<class F>
 __device__ __forceinline__ float over_lane_groups(float x, F combine) {
@@ -103,7 +111,7 @@ __device__ __forceinline__ float over_lane_groups(float x, F combine) {
     return combine(as_float((int)b[0]), as_float((int)b[1]));
 }
 __device__ __forceinline__ float max_over_lane_groups(float x) {
-    return over_lane_groups(x, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    return over_lane_groups(x, [](float a, float b) { return larger(a, b); });
 }
 __device__ __forceinline__ float sum_over_lane_groups(float x) {
     return over_lane_groups(x, [](float a, float b) { return a + b; });
@@ -271,12 +279,12 @@ struct RowState {
             float top = kLowest;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const float most = __builtin_fmaxf(__builtin_fmaxf(s[r][t][0], s[r][t][1]), __builtin_fmaxf(s[r][t][2], s[r][t][3]));
-                top = __builtin_fmaxf(top, __builtin_fmaf(most, scales[t].k, scales[t].up));
+                const float most = larger(larger(s[r][t][0], s[r][t][1]), larger(s[r][t][2], s[r][t][3]));
+                top = larger(top, __builtin_fmaf(most, scales[t].k, scales[t].up));
             }
             top = max_over_lane_groups(top);
             if (__ballot(top > m[r]) != 0) {
-                const float now = __builtin_fmaxf(top, m[r]);
+                const float now = larger(top, m[r]);
                 const float shrink = __builtin_amdgcn_exp2f(m[r] - now);
                 m[r] = now;
                 l[r] *= shrink;
@@ -545,9 +553,11 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
 // instructions take, a 16-key tile by each wavefront: codes are converted and
 // values transposed once for the whole workgroup, and fragments are read 16 bytes
 // a lane without bank conflicts.  The next block's codes are loaded while this one
-// is multiplied; two buffers, one barrier a block.  Bound by the vector ALU: per
-// 16 rows and 32 keys a softmax of 8 scores a lane (8 exponentials at a quarter of
-// the rate) stands against D / 8 matrix instructions.
+// is multiplied.  Bound by the vector ALU: per 16 rows and 32 keys a softmax of 8
+// scores a lane (8 exponentials at a quarter of the rate) stands against D / 8 matrix
+// instructions.  6 requests of 113 to 447 queries and 4032 to 5915 keys, 16 heads of
+// 64 on 4: 30.6 GFLOP in 97 us, 15 of them the join of six splits (213 us with keys
+// from memory for every wavefront).
 template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, class T>
 __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
     constexpr int kRows = 16 * R, kTileRows = kRows * WAVES, kBlock = 16 * WAVES;
@@ -559,9 +569,11 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
     const int tiles = (int)to.pieces / request.splits;
     const float scale = __builtin_fabsf(batch.scale);
 
-    __shared__ __attribute__((aligned(16))) uint32_t k_frags[2][WAVES][D / 32][kWaveSize][4];
-    __shared__ __attribute__((aligned(16))) uint32_t v_frags[2][WAVES / 2][D / 16][kWaveSize][4];
-    __shared__ __attribute__((aligned(16))) float tile_scales[2][WAVES][4];  // k, up, per_v, there
+    // Two buffers and one barrier a block; one and two where two would leave no room in LDS for a second workgroup.
+    constexpr int kBuffers = D <= 128 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) uint32_t k_frags[kBuffers][WAVES][D / 32][kWaveSize][4];
+    __shared__ __attribute__((aligned(16))) uint32_t v_frags[kBuffers][WAVES / 2][D / 16][kWaveSize][4];
+    __shared__ __attribute__((aligned(16))) float tile_scales[kBuffers][WAVES][4];  // k, up, per_v, there
 
     for (int tile = (int)piece.x / request.splits; tile * kTileRows < request.rows; tile += tiles) {
         const int row0 = tile * kTileRows + wave * kRows;
@@ -609,7 +621,7 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
             stage(0, base + 16 * wave);
         }
         __syncthreads();
-        for (int buffer = 0; base < end; buffer ^= 1) {
+        for (int buffer = 0; base < end; buffer ^= kBuffers - 1) {
             const bool more = base + kBlock < end;
             if (more) {
                 walk.load_keys(keys, base + kBlock + 16 * wave, id);
@@ -643,8 +655,11 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
                         });
                 }
             }
+            if (kBuffers == 1) {
+                __syncthreads();  // this block has been read
+            }
             if (more) {
-                stage(buffer ^ 1, base + kBlock + 16 * wave);
+                stage(buffer ^ (kBuffers - 1), base + kBlock + 16 * wave);
             }
             __syncthreads();
             base += kBlock;
@@ -683,9 +698,11 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
     }
 }
 
-// Rows of the result from the splits' parts: one workgroup a row, whose
-// wavefronts take the splits (at most 256) in turn and meet in LDS, always in the
-// same order.  A lane first holds the statistics of splits lane, lane + 64 ...
+// Rows of the result from the splits' parts: PER_ROW wavefronts a row take the
+// splits (at most 64 for one wavefront, 256 for a workgroup) in turn and meet in LDS,
+// always in the same order.  A lane first holds the statistics of splits lane,
+// lane + 64 ...  One wavefront a row pays for many rows of few splits (25472 rows, 6
+// splits, 64 dimensions: 35 us with four), four for few rows of many.
 constexpr int kSplitsPerLane = 4;
 struct JoinRows {
     uint32_t *out;
@@ -693,7 +710,8 @@ struct JoinRows {
     const float *partial, *stats;
     const int32_t *starts;
     int64_t splits, requests, q_heads;
-    int64_t rows;  // tokens * query heads: workgroups
+    int64_t rows;    // tokens * query heads
+    int64_t blocks;  // workgroups
 
     __device__ __forceinline__ struct JoinBlock block(int64_t x) const;
 };
@@ -705,19 +723,22 @@ __device__ __forceinline__ JoinBlock JoinRows::block(int64_t x) const {
     return {*this, x};
 }
 
-template<int64_t D, int64_t WAVES, class T>
+template<int64_t D, int64_t WAVES, int64_t PER_ROW, class T>
 __device__ __forceinline__ void join_splits(const AttentionBatchOf<T> &, const JoinBlock &block) {
     constexpr int kPart = D / 64;  // values a lane
+    constexpr int kHeld = PER_ROW == 1 ? 1 : kSplitsPerLane;
+    static_assert(PER_ROW == 1 || PER_ROW == WAVES, "a row is a wavefront's or the workgroup's");
     const JoinRows &to = block.to;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
-    const int64_t row = block.x, token = row / to.q_heads;
-    if (token < to.starts[0] || token >= to.starts[to.requests]) {
+    const int row = (int)(block.x * (WAVES / PER_ROW)) + (PER_ROW == 1 ? wave : 0), token = row / (int)to.q_heads;
+    // a row of no request has no parts
+    if (row >= (int)to.rows || token < to.starts[0] || token >= to.starts[to.requests]) {
         return;
     }
     const int splits = (int)to.splits;
-    float m[kSplitsPerLane], l[kSplitsPerLane], top = detail::kLowest;
+    float m[kHeld], l[kHeld], top = detail::kLowest;
 #pragma unroll
-    for (int j = 0; j < kSplitsPerLane; j++) {
+    for (int j = 0; j < kHeld; j++) {
         const int s = j * kWaveSize + lane;
         m[j] = detail::kLowest, l[j] = 0.0f;
         if (s < splits) {
@@ -729,53 +750,70 @@ __device__ __forceinline__ void join_splits(const AttentionBatchOf<T> &, const J
     for (int d = 1; d < kWaveSize; d *= 2) {
         top = __builtin_fmaxf(top, __shfl_xor(top, d));
     }
-    __shared__ float weights[kSplitsPerLane * kWaveSize];
-    float sum = 0.0f;
+    float weight[kHeld], sum = 0.0f;
     int used = 0;  // splits up to the last one that saw any of the row's keys
 #pragma unroll
-    for (int j = 0; j < kSplitsPerLane; j++) {
-        const float weight = l[j] != 0.0f ? __builtin_amdgcn_exp2f(m[j] - top) : 0.0f;
-        sum = __builtin_fmaf(l[j], weight, sum);
-        weights[j * kWaveSize + lane] = weight;  // every wavefront writes the same
+    for (int j = 0; j < kHeld; j++) {
+        weight[j] = l[j] != 0.0f ? __builtin_amdgcn_exp2f(m[j] - top) : 0.0f;
+        sum = __builtin_fmaf(l[j], weight[j], sum);
         const uint64_t some = __ballot(l[j] != 0.0f);
         used = some != 0 ? j * kWaveSize + 64 - __builtin_clzll(some) : used;
     }
     for (int d = 1; d < kWaveSize; d *= 2) {
         sum += __shfl_xor(sum, d);
     }
-    __syncthreads();
+    const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
     float x[kPart];
 #pragma unroll
     for (int i = 0; i < kPart; i++) {
         x[i] = 0.0f;
     }
-    const float *part = to.partial + row * D + lane * kPart;
-#pragma unroll 8
-    for (int s = wave; s < used; s += WAVES) {
-        const float w = weights[s];
+    const float *part = to.partial + (int64_t)row * D + lane * kPart;
+    uint32_t *out = to.out + token * to.out_pitch + (row % (int)to.q_heads) * (D / 2);
+    auto add = [&](int s, float w) {
 #pragma unroll
         for (int i = 0; i < kPart; i++) {
             // a split without any of the row's keys wrote no part
             const float p = part[s * to.rows * D + i];
             x[i] = __builtin_fmaf(w != 0.0f ? p : 0.0f, w, x[i]);
         }
-    }
-    __shared__ float parts[WAVES][D];
-#pragma unroll
-    for (int i = 0; i < kPart; i++) {
-        parts[wave][lane * kPart + i] = x[i];
-    }
-    __syncthreads();
-    const float per_sum = sum != 0.0f ? 1.0f / sum : 0.0f;
-    uint32_t *out = to.out + token * to.out_pitch + (row % to.q_heads) * (D / 2);
-    if (threadIdx.x < D / 2) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            a += parts[w][2 * threadIdx.x];
-            b += parts[w][2 * threadIdx.x + 1];
+    };
+    if constexpr (PER_ROW == 1) {
+#pragma unroll 4
+        for (int s = 0; s < used; s++) {
+            add(s, as_float(__builtin_amdgcn_readlane(as_int(weight[0]), s)));
         }
-        out[threadIdx.x] = pack_halves<T>(a * per_sum, b * per_sum);
+        unsigned short *to_lane = reinterpret_cast<unsigned short *>(out) + lane * kPart;
+#pragma unroll
+        for (int i = 0; i < kPart; i++) {
+            to_lane[i] = (unsigned short)(pack_halves<T>(x[i] * per_sum, 0.0f) & 0xffffu);
+        }
+    } else {
+        __shared__ float weights[kHeld * kWaveSize];
+        __shared__ float parts[WAVES][D];
+#pragma unroll
+        for (int j = 0; j < kHeld; j++) {
+            weights[j * kWaveSize + lane] = weight[j];  // every wavefront writes the same
+        }
+        __syncthreads();
+#pragma unroll 8
+        for (int s = wave; s < used; s += WAVES) {
+            add(s, weights[s]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPart; i++) {
+            parts[wave][lane * kPart + i] = x[i];
+        }
+        __syncthreads();
+        if (threadIdx.x < D / 2) {
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                a += parts[w][2 * threadIdx.x];
+                b += parts[w][2 * threadIdx.x + 1];
+            }
+            out[threadIdx.x] = pack_halves<T>(a * per_sum, b * per_sum);
+        }
     }
 }
 
