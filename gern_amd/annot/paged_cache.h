@@ -16,7 +16,7 @@ struct PagedCache {
     uint32_t *faults;
 };
 struct WritableCache : PagedCache {
-    int64_t stretches, stretch, sides;
+    int64_t pieces, stretch;
 };
 struct NewTokens {
     const void *k, *v;

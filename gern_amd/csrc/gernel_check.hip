@@ -168,7 +168,7 @@ template __global__ void check_page_table<8>(gernels::RequestLengths, gernels::F
 
 template<int64_t D, int64_t PAGE, int64_t THREADS, class T>
 __global__ void __launch_bounds__(THREADS) check_write_cache(gernels::NewTokensOf<T> tokens, gernels::WritableCache cache) {
-    auto stretch = cache.at(blockIdx.x, blockIdx.y, blockIdx.z);
+    auto stretch = cache.at(blockIdx.x);
     gernels::write_cache<D, PAGE, THREADS>(tokens.whole(), stretch);
 }
 template __global__ void check_write_cache<128, 16, 64, gernels::Bf16>(gernels::NewTokensOf<gernels::Bf16>, gernels::WritableCache);
