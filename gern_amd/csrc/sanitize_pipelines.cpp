@@ -55,6 +55,25 @@ int main() {
             gern_pipeline_destroy(p);
         }
         expect(gern_gemm_schedule_create(4, compile_only, &p) != 0 && p == nullptr, "bad schedule");
+        expect(gern_page_table_create(32, compile_only, &p) == 0, "page table create");
+        gern_pipeline_destroy(p);
+        for (int type : {(int)GERN_TYPE_BF16, (int)GERN_TYPE_F16}) {
+            expect(gern_cache_write_create(64, 16, type, compile_only, &p) == 0, "cache write create");
+            gern_pipeline_destroy(p);
+            expect(gern_cache_attention_create(192, 128, type, compile_only, &p) == 0, "cache attention create");
+            int64_t bytes = -1, faults = -1;
+            expect(gern_cache_attention_workspace(p, 3, 2, 8, 2, 1, 100000, &bytes) == 0 && bytes > 0, "workspace");
+            expect(gern_cache_attention_workspace(p, 3, 2, 7, 2, 1, 100000, &bytes) != 0, "heads that do not divide");
+            expect(gern_pipeline_faults(p, &faults) == 0 && faults == 0, "no faults without a run");
+            gern_pipeline_destroy(p);
+            expect(gern_matvec4_create(32, type, compile_only, &p) == 0, "matvec create");
+            uint8_t byte = 0;
+            expect(gern_matvec4_run(p, &byte, 32, &byte, &byte, nullptr, &byte, 1, 1, 1, 32, nullptr) != 0, "compile-only pipeline must refuse to run");
+            gern_pipeline_destroy(p);
+        }
+        expect(gern_page_table_create(17, compile_only, &p) != 0 && p == nullptr, "bad page size");
+        expect(gern_cache_attention_create(100, 16, 0, compile_only, &p) != 0 && p == nullptr, "bad head dimension");
+        expect(gern_matvec4_create(128, 3, compile_only, &p) != 0 && p == nullptr, "bad type");
         // argument errors leave no pipeline behind
         expect(gern_gemm_create(7, compile_only, &p) != 0 && p == nullptr, "bad variant");
         expect(gern_softmax_create(0, 1, compile_only, &p) != 0 && p == nullptr, "bad width");

@@ -779,9 +779,12 @@ __device__ __forceinline__ void join_splits(const AttentionBatchOf<T> &, const J
         }
     };
     if constexpr (PER_ROW == 1) {
-#pragma unroll 4
+        // through LDS and not from lane to lane, so that the loop unrolls and its loads overlap; only this wavefront reads
+        __shared__ float weights[WAVES][kWaveSize];
+        weights[wave][lane] = weight[0];
+#pragma unroll 8
         for (int s = 0; s < used; s++) {
-            add(s, as_float(__builtin_amdgcn_readlane(as_int(weight[0]), s)));
+            add(s, weights[wave][s]);
         }
         unsigned short *to_lane = reinterpret_cast<unsigned short *>(out) + lane * kPart;
 #pragma unroll

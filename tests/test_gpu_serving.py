@@ -403,29 +403,46 @@ def test_attention_length_beyond_the_table(torch, gpu):
 
 
 def test_a_serving_step(torch, gpu):
-    """Tables, write and attention as a server calls them: prompts, then tokens one at a time, replayed from a graph."""
-    dim, page, heads, group, requests, pages = 128, 16, 2, 4, 3, 40
+    """All operators as a server calls them: projection, tables, write, attention, projection; prompts, then tokens one at a
+    time, replayed from a graph in turn with eager calls."""
+    dim, page, heads, group, requests, pages, hidden, columns = 128, 16, 2, 4, 3, 40, 256, 64
     rs = np.random.RandomState(12)
-    tables, write, attend = (gpu(n, **k) for n, k in (("PageTable", dict(page_size=page)), ("CacheWrite", dict(head_dim=dim, page_size=page, dtype="bf16")),
-                                                      ("CacheAttention", dict(head_dim=dim, page_size=page, dtype="bf16"))))
-    width, most = 12, 60
+    tables, write, attend, project = (gpu(n, **k) for n, k in (
+        ("PageTable", dict(page_size=page)), ("CacheWrite", dict(head_dim=dim, page_size=page, dtype="bf16")),
+        ("CacheAttention", dict(head_dim=dim, page_size=page, dtype="bf16")), ("Matvec4", dict(group=columns, dtype="bf16"))))
+    width, most, qkv_rows = 12, 60, heads * (group + 2)
     state = dict(cached=i32(torch, [0] * requests), added=i32(torch, [0] * requests), free=i32(torch, rs.permutation(pages)), count=i32(torch, [pages]),
                  table=i32(torch, np.full((requests, width), -1)), lengths=i32(torch, [0] * requests), starts=i32(torch, [0] * (requests + 1)),
                  slots=i32(torch, [0] * most), counts=i32(torch, [0, 0]))
     kc, vc = (torch.full((pages, heads, page, dim), 127, dtype=torch.uint8, device="cuda") for _ in range(2))
     ks, vs = (torch.full((pages, heads), float("nan"), device="cuda") for _ in range(2))
-    qkv = torch.zeros((most, heads * (group + 2), dim), dtype=torch.bfloat16, device="cuda")
+
+    def weights(n, k):
+        return (torch.from_numpy(rs.randint(0, 256, (n, k // 2)).astype(np.uint8)).cuda(),
+                torch.from_numpy(rs.uniform(0.005, 0.02, (k // columns, n))).bfloat16().cuda(),
+                torch.from_numpy(rs.randint(4, 12, (k // columns, n)).astype(np.uint8)).cuda())
+
+    def check_product(x, w, y):
+        want, tol = so.matvec4(x.double().cpu().numpy(), w[0].cpu().numpy(), w[1].double().cpu().numpy(), w[2].double().cpu().numpy(), columns, 128)
+        assert np.all(np.abs(y.double().cpu().numpy() - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol))
+
+    w_in, w_out = weights(qkv_rows * dim, hidden), weights(hidden, heads * group * dim)
+    x = torch.zeros((most, hidden), dtype=torch.bfloat16, device="cuda")
+    qkv = torch.zeros((most, qkv_rows, dim), dtype=torch.bfloat16, device="cuda")
     out = torch.zeros((most, heads * group, dim), dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((most, hidden), dtype=torch.bfloat16, device="cuda")
     ws = torch.zeros(attend.workspace_bytes(most, requests, heads * group, heads, most, width * page), dtype=torch.uint8, device="cuda")
     side = torch.cuda.Stream()
 
     def step(stream):
         q, k, v = qkv[:, :heads * group], qkv[:, heads * group:heads * (group + 1)], qkv[:, heads * (group + 1):]
+        project(x, w_in[0], w_in[1], qkv.view(most, -1), zeros=w_in[2], stream=stream)
         tables(state["cached"], state["added"], state["free"], state["count"], state["table"], state["lengths"], state["starts"], state["slots"],
                state["counts"], stream=stream)
         write(k, v, state["slots"], kc, vc, ks, vs, stream=stream)
         attend(q, kc, vc, ks, vs, state["table"], state["lengths"], state["starts"], out, dim ** -0.5, max_queries=most, max_length=width * page, workspace=ws,
                stream=stream)
+        project(out.view(most, -1), w_out[0], w_out[1], y, zeros=w_out[2], stream=stream)
 
     with torch.cuda.stream(side):
         step(side.cuda_stream)  # adds nothing: no request has tokens yet
@@ -437,9 +454,10 @@ def test_a_serving_step(torch, gpu):
     keys = [[np.zeros((0, heads, dim))] * 2 for _ in range(requests)]  # of each request, before they are coded
     for turn, added in enumerate([[20, 1, 33], [1, 1, 1], [1, 0, 1], [1, 16, 1], [14, 1, 0], [1, 1, 1]]):
         state["added"].copy_(i32(torch, added))
-        fresh = rs.normal(size=tuple(qkv.shape))
-        qkv.copy_(torch.from_numpy(fresh).bfloat16())
+        x.copy_(torch.from_numpy(rs.normal(size=tuple(x.shape))).bfloat16())
         out.fill_(5.0)
+        for t in (qkv, y):
+            t.fill_(float("nan"))
         torch.cuda.synchronize()
         if turn % 2 == 0:
             graph.replay()
@@ -447,15 +465,17 @@ def test_a_serving_step(torch, gpu):
             step(None)
         torch.cuda.synchronize()
         assert int(state["counts"][1]) == 0 and write.faults() == 0 and attend.faults() == 0
+        check_product(x, w_in, qkv.view(most, -1))
+        check_product(out.view(most, -1), w_out, y)
         starts = np.concatenate([[0], np.cumsum(added)])
         assert np.array_equal(state["starts"].cpu().numpy(), starts)
-        x = qkv.double().cpu().numpy()
+        values = qkv.double().cpu().numpy()
         got = out.double().cpu().numpy()
         assert np.all(got[starts[-1]:] == 5.0)
         scales = [ks.cpu().numpy().astype(np.float64), vs.cpu().numpy().astype(np.float64)]
         table = state["table"].cpu().numpy()
         for b in range(requests):
-            mine = x[starts[b]:starts[b + 1]]
+            mine = values[starts[b]:starts[b + 1]]
             for side_of in (0, 1):
                 at = heads * (group + side_of)
                 keys[b][side_of] = np.concatenate([keys[b][side_of], mine[:, at:at + heads]])
@@ -478,52 +498,36 @@ def test_a_serving_step(torch, gpu):
         state["count"].copy_(state["counts"][:1])
 
 
-# ------------------------------------------------------------------------------------------------ 4-bit weights
-
-def run_matvec(torch, gpu, dtype, group, m, n, k, zeros="random", seed=0, mean=0.0):
-    rs = np.random.RandomState(seed + m + n + k)
-    t = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
-    x = torch.from_numpy(rs.normal(size=(m, k + 8)) + mean).to(t)
-    codes = rs.randint(0, 256, (n, k // 2)).astype(np.uint8)
-    scales = torch.from_numpy(rs.uniform(0.005, 0.02, (k // group, n)) * rs.choice([-1.0, 1.0], (k // group, n))).to(t)
-    z = {"random": rs.randint(0, 16, (k // group, n)), "wide": rs.randint(0, 256, (k // group, n)), "none": np.full((k // group, n), 8)}[zeros].astype(np.uint8)
-    y = torch.full((m, n + 3), 99.0, dtype=t, device="cuda")  # rows of x and y stand in wider ones
-    gpu("Matvec4", group=group, dtype=dtype)(x.cuda()[:, :k], torch.from_numpy(codes).cuda(), scales.cuda(), y[:, :n],
-                                             zeros=None if zeros == "none" else torch.from_numpy(z).cuda())
+def test_two_streams_at_a_time(torch, gpu):
+    """One pipeline on two streams, each with its own buffers and workspace; the same results as one after the other."""
+    a = gpu("CacheAttention", head_dim=128, page_size=16, dtype="bf16")
+    runs = []
+    for seed in (20, 21):
+        device, host, out = attention_inputs(torch, "bf16", 128, 16, 2, 4, [5000, 300], [1, 2], seed=seed)
+        n = a.workspace_bytes(device["q"].shape[0], 2, 8, 2, 2, 5000)
+        runs.append((device, host, out, torch.empty(n, dtype=torch.uint8, device="cuda"), torch.cuda.Stream()))
     torch.cuda.synchronize()
-    got = y.double().cpu().numpy()
-    assert np.all(got[:, n:] == 99.0)
-    want, tol = so.matvec4(x[:, :k].double().numpy(), codes, scales.double().numpy(), z.astype(np.float64), group, {"bf16": 128, "f16": 64}[dtype])
-    tol = tol + HALF_STEP[dtype] * (np.abs(want) + tol) + 2.0 ** -25
-    assert np.all(np.abs(got[:, :n] - want) <= tol), float((np.abs(got[:, :n] - want) / tol).max())
+    for _ in range(5):
+        for device, _, _, ws, stream in runs:
+            a(**device, scale=0.1, max_queries=2, max_length=5000, workspace=ws, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for _, host, out, _, _ in runs:
+        check_attention(out, host, "bf16", 16, 4, 0.1)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 16, 3), (2, 17, 8), (15, 33, 9), (16, 100, 2), (17, 31, 5), (33, 64, 4), (64, 129, 7), (1, 1000, 33)])
-def test_matvec(torch, gpu, dtype, group, m, n, k):
-    """k in groups: blocks of 128 columns that are whole, partial, and fewer than the wavefronts."""
-    run_matvec(torch, gpu, dtype, group, m, n, k * group, seed=group)
-
-
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("m, n, k, zeros", [(1, 20000, 256, "none"), (5, 16385, 128, "wide"), (1, 48, 16384, "random"), (40, 300, 4096, "none"), (64, 5, 8192, "wide")])
-def test_matvec_sizes(torch, gpu, dtype, m, n, k, zeros):
-    run_matvec(torch, gpu, dtype, 128, m, n, k, zeros=zeros)
-
-
-def test_matvec_activations_with_a_mean(torch, gpu):
-    """The sums that the offset and the zero point take out are large then."""
-    for dtype in ("bf16", "f16"):
-        run_matvec(torch, gpu, dtype, 64, 3, 65, 2048, mean=4.0)
-
-
-def test_matvec_row_with_nan_stays_alone(torch, gpu):
-    rs = np.random.RandomState(1)
-    x = torch.from_numpy(rs.normal(size=(3, 256))).bfloat16().cuda()
-    x[1, 77] = float("nan")
-    codes, scales = torch.from_numpy(rs.randint(0, 256, (40, 128)).astype(np.uint8)).cuda(), torch.full((2, 40), 0.01, dtype=torch.bfloat16, device="cuda")
-    y = torch.zeros((3, 40), dtype=torch.bfloat16, device="cuda")
-    gpu("Matvec4", group=128, dtype="bf16")(x, codes, scales, y)
-    assert torch.isnan(y[1]).all() and torch.isfinite(y[::2]).all()
-    gpu("Matvec4", group=128, dtype="bf16")(x[:0], codes, scales, y[:0])
+@pytest.mark.parametrize("dim, scale", [(64, -0.2), (128, 0.0), (192, -0.05), (256, 0.5)])
+def test_attention_scales_of_any_sign(torch, gpu, dim, scale):
+    for queries in (2, 70):
+        device, host, out = attention_inputs(torch, "f16", dim, 32, 1, 3, [120, 33], [queries, 1], seed=dim)
+        a = gpu("CacheAttention", head_dim=dim, page_size=32, dtype="f16")
+        a(**device, scale=scale, max_queries=queries, max_length=120)
+        torch.cuda.synchronize()
+        o, starts = out.double().cpu().numpy(), host["starts"]
+        for b, n in enumerate(host["lengths"]):
+            pages, m = host["table"][b, :-(-n // 32)], starts[b + 1] - starts[b]
+            k, v = ((host["codes"][s][pages, 0] * host["scales"][s][pages, 0][:, None, None]).reshape(-1, dim)[:n] for s in (0, 1))
+            vs = np.repeat(host["scales"][1][pages, 0], 32)[:n]
+            for u in range(3):
+                q = host["q"][starts[b]:starts[b + 1], u]
+                want, tol = so.attention(np.sign(scale) * q, k, v, vs, n - m + np.arange(m) + 1, abs(scale))
+                assert np.all(np.abs(o[starts[b]:starts[b + 1], u] - want) <= tol + HALF_STEP["f16"] * (np.abs(want) + tol) + 2.0 ** -25)
