@@ -358,7 +358,7 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     plan.variant = rows <= 64 ? 0 : 1;
     const int64_t tile = plan.variant == 0 ? 16 : 16 * kAttentionWaves * attentionRowTiles(head_dim);
     plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
-    // Keys are split, into pieces of at least 256, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
+    // Keys are split, into pieces of at least 512, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
     // to three times what is resident, so that requests of different lengths leave few CUs idle at the end.  Few rows of
     // more than 128 dimensions: two, what is resident, because the joined parts are larger and a start costs more.
     // Measured (us) with 512 / 1024 / 2048 / 4096: 64 requests of 4096 to 8192 keys, 8 heads of 128: 181 / 175 / 155 /
@@ -367,9 +367,11 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     const int64_t wanted = plan.variant == 0 && head_dim > 128 ? 512 : 2048;
     const int64_t whole = requests * heads * plan.row_tiles;
     // Up to 1024 keys are not worth a second launch (1 request of 700, 8 heads of 128: 10.4 us whole, 13.9 split; 1000:
-    // 12.3, 11.9; 2000: 18.6, 13.4).
-    const int64_t splits = max_length <= 1024 ? 1 : std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
-    plan.chunk = std::max<int64_t>(256, ((max_length + splits - 1) / splits + 255) / 256 * 256);
+    // 12.3, 11.9; 2000: 18.6, 13.4), nor are workgroups for every CU four times over (128 requests of 1000 to 2000, 8 heads
+    // of 128: 87 whole, 97 in two).  Pieces of 256 / 512 / 1024 at least: 16 requests of 2000 to 4000 33.3 / 31.7 / 27.5, one
+    // of 32768 18.4 / 17.1 / 19.5, two of 20000, 4 heads 16.0 / 15.8 / 18.6.
+    const int64_t splits = max_length <= 1024 || whole >= 1024 ? 1 : std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
+    plan.chunk = std::max<int64_t>(512, ((max_length + splits - 1) / splits + 255) / 256 * 256);
     plan.splits = std::max<int64_t>(1, (max_length + plan.chunk - 1) / plan.chunk);
     // BLOCK_Y holds 65535 pieces; a workgroup takes further row tiles in turn
     plan.row_tiles = std::min(plan.row_tiles, 65535 / plan.splits);

@@ -335,7 +335,7 @@ __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const W
     };
 
     int block = wave;
-    if constexpr (MT <= 1) {
+    if constexpr (MT <= 1 || NT == 1) {
         // The next block's loads are issued in front of this one's products, and the barriers keep them there.
         if (block < blocks) {
             Block even, odd;

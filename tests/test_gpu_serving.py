@@ -399,6 +399,57 @@ def test_attention_length_beyond_the_table(torch, gpu):
     check_attention(out, host, "bf16", 16, 1, 0.125)
 
 
+# ------------------------------------------------------------------------------------------------ 4-bit weights
+
+def run_matvec(torch, gpu, dtype, group, m, n, k, zeros="random", seed=0, mean=0.0):
+    rs = np.random.RandomState(seed + m + n + k)
+    t = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    x = torch.from_numpy(rs.normal(size=(m, k + 8)) + mean).to(t)
+    codes = rs.randint(0, 256, (n, k // 2)).astype(np.uint8)
+    scales = torch.from_numpy(rs.uniform(0.005, 0.02, (k // group, n)) * rs.choice([-1.0, 1.0], (k // group, n))).to(t)
+    z = {"random": rs.randint(0, 16, (k // group, n)), "wide": rs.randint(0, 256, (k // group, n)), "none": np.full((k // group, n), 8)}[zeros].astype(np.uint8)
+    y = torch.full((m, n + 3), 99.0, dtype=t, device="cuda")  # rows of x and y stand in wider ones
+    gpu("Matvec4", group=group, dtype=dtype)(x.cuda()[:, :k], torch.from_numpy(codes).cuda(), scales.cuda(), y[:, :n],
+                                             zeros=None if zeros == "none" else torch.from_numpy(z).cuda())
+    torch.cuda.synchronize()
+    got = y.double().cpu().numpy()
+    assert np.all(got[:, n:] == 99.0)
+    want, tol = so.matvec4(x[:, :k].double().numpy(), codes, scales.double().numpy(), z.astype(np.float64), group, {"bf16": 128, "f16": 64}[dtype])
+    tol = tol + HALF_STEP[dtype] * (np.abs(want) + tol) + 2.0 ** -25
+    assert np.all(np.abs(got[:, :n] - want) <= tol), float((np.abs(got[:, :n] - want) / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 16, 3), (2, 17, 8), (15, 33, 9), (16, 100, 2), (17, 31, 5), (33, 64, 4), (64, 129, 7), (1, 1000, 33)])
+def test_matvec(torch, gpu, dtype, group, m, n, k):
+    """k in groups: blocks of 128 columns that are whole, partial, and fewer than the wavefronts."""
+    run_matvec(torch, gpu, dtype, group, m, n, k * group, seed=group)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m, n, k, zeros", [(1, 20000, 256, "none"), (5, 16385, 128, "wide"), (1, 48, 16384, "random"), (40, 300, 4096, "none"), (64, 5, 8192, "wide")])
+def test_matvec_sizes(torch, gpu, dtype, m, n, k, zeros):
+    run_matvec(torch, gpu, dtype, 128, m, n, k, zeros=zeros)
+
+
+def test_matvec_activations_with_a_mean(torch, gpu):
+    """The sums that the offset and the zero point take out are large then."""
+    for dtype in ("bf16", "f16"):
+        run_matvec(torch, gpu, dtype, 64, 3, 65, 2048, mean=4.0)
+
+
+def test_matvec_row_with_nan_stays_alone(torch, gpu):
+    rs = np.random.RandomState(1)
+    x = torch.from_numpy(rs.normal(size=(3, 256))).bfloat16().cuda()
+    x[1, 77] = float("nan")
+    codes, scales = torch.from_numpy(rs.randint(0, 256, (40, 128)).astype(np.uint8)).cuda(), torch.full((2, 40), 0.01, dtype=torch.bfloat16, device="cuda")
+    y = torch.zeros((3, 40), dtype=torch.bfloat16, device="cuda")
+    gpu("Matvec4", group=128, dtype="bf16")(x, codes, scales, y)
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[::2]).all()
+    gpu("Matvec4", group=128, dtype="bf16")(x[:0], codes, scales, y[:0])
+
+
 # ------------------------------------------------------------------------------------------------ a step
 
 
