@@ -1,4 +1,4 @@
-// Host mirrors of the aggregates of gernels/matvec4.h; the annotations are the
+// Host mirrors of the aggregates of gernels/serving/matvec4.h; the annotations are the
 // general ones of annot/pieces.h.
 #pragma once
 

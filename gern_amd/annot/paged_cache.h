@@ -1,5 +1,5 @@
 // Host mirrors of the aggregates of the gernels over a paged 8-bit cache of keys
-// and values (gernels/paged_cache.h, page_table.h, cache_write.h,
+// and values (gernels/serving/paged_cache.h, page_table.h, cache_write.h,
 // cache_attention.h); the annotations are the general ones of annot/pieces.h.
 #pragma once
 

@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(512) check_qk_softmax_tiles(gernels::MatrixBF1
 template __global__ void check_qk_softmax_tiles<128>(gernels::MatrixBF16, gernels::MatrixBF16, gernels::MatrixF32, gernels::RowStatsExchange, float);
 template __global__ void check_qk_softmax_tiles<192>(gernels::MatrixBF16, gernels::MatrixBF16, gernels::MatrixF32, gernels::RowStatsExchange, float);
 
-#include "gernels/cache_attention.h"
-#include "gernels/cache_write.h"
-#include "gernels/page_table.h"
+#include "gernels/serving/cache_attention.h"
+#include "gernels/serving/cache_write.h"
+#include "gernels/serving/page_table.h"
 
 template<int64_t PER>
 __global__ void __launch_bounds__(1024) check_page_table(gernels::RequestLengths batch, gernels::FreePages free_pages, gernels::PageTableOut table) {
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) check_join_splits(gernels::AttentionBatch
 template __global__ void check_join_splits<192, 4, gernels::Bf16>(gernels::AttentionBatchOf<gernels::Bf16>, gernels::JoinRows);
 template __global__ void check_join_splits<64, 1, gernels::F16>(gernels::AttentionBatchOf<gernels::F16>, gernels::JoinRows);
 
-#include "gernels/matvec4.h"
+#include "gernels/serving/matvec4.h"
 
 template<int64_t G, int64_t MT, int64_t NT, class T>
 __global__ void __launch_bounds__(512) check_matvec4(gernels::ActivationsOf<T> x, gernels::Weights4 weights, gernels::MatvecOut y) {

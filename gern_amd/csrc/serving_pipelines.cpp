@@ -159,7 +159,7 @@ int gern_page_table_create(int64_t page_size, int flags, gern_pipeline *out) {
             AbstractDataTypePtr free_pages(new const annot::WholeADT("free_pages", "gernels::FreePages"));
             AbstractDataTypePtr table(
                 new const annot::PiecesADT<hip::PageTableOut>("table", "gernels::PageTableOut", "share", {{"shares", &hip::PageTableOut::shares}}));
-            annot::PieceFunction extend("gernels::extend_page_table", "gernels/page_table.h", {batch, free_pages}, table, {"shares"},
+            annot::PieceFunction extend("gernels::extend_page_table", "gernels/serving/page_table.h", {batch, free_pages}, table, {"shares"},
                                         {"page", "threads", "per"});
             Variable one("one"), threads("block");
             Composable program = Global((Tile(table["shares"], one.bind(1)) || Grid::BLOCK_X)(
@@ -267,7 +267,7 @@ int gern_cache_write_create(int64_t head_dim, int64_t page_size, int type, int f
             AbstractDataTypePtr tokens(new const annot::WholeADT("tokens", "gernels::NewTokensOf<" + typeName(type) + ">"));
             using Cache = hip::WritableCache;
             AbstractDataTypePtr cache(new const annot::PiecesADT<Cache>("cache", "gernels::WritableCache", "at", {{"pieces", &Cache::pieces}}));
-            annot::PieceFunction write("gernels::write_cache", "gernels/cache_write.h", {tokens}, cache, {"pieces"}, {"head_dim", "page", "threads"});
+            annot::PieceFunction write("gernels::write_cache", "gernels/serving/cache_write.h", {tokens}, cache, {"pieces"}, {"head_dim", "page", "threads"});
             Variable x("x"), block("block");
             Composable program = Global((Tile(cache["pieces"], x.bind(1)) || Grid::BLOCK_X)(write[{constant("head_dim", head_dim), constant("page", page_size),
                                                                                                    constant("threads", threads)}](tokens, cache)),
@@ -334,7 +334,7 @@ struct AttentionPlan {
     int64_t row_tiles, splits, chunk;
 };
 
-constexpr int64_t kMaxSplits = 256;  // gernels/cache_attention.h, join_splits
+constexpr int64_t kMaxSplits = 256;  // gernels/serving/cache_attention.h, join_splits
 
 // The programs of a pipeline, four wavefronts a workgroup: few rows (queries times the heads that share a head of the
 // cache) against keys that the wavefronts divide, or many rows divided among the wavefronts.
@@ -414,7 +414,7 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
         Draft p(gern_pipeline_s::CACHE_ATTENTION, flags);
         p->head_dim = head_dim;
         p->page_size = page_size;
-        const std::string header = "gernels/cache_attention.h", batch_type = "gernels::AttentionBatchOf<" + typeName(type) + ">";
+        const std::string header = "gernels/serving/cache_attention.h", batch_type = "gernels::AttentionBatchOf<" + typeName(type) + ">";
         AbstractDataTypePtr batch(new const annot::WholeADT("batch", batch_type));
         AbstractDataTypePtr cache(new const annot::WholeADT("cache", "gernels::PagedCache"));
         for (bool few : {true, false}) {
@@ -589,7 +589,7 @@ int gern_matvec4_create(int64_t group, int type, int flags, gern_pipeline *out) 
             AbstractDataTypePtr x(new const annot::WholeADT("x", "gernels::ActivationsOf<" + typeName(type) + ">"));
             AbstractDataTypePtr weights(new const annot::WholeADT("weights", "gernels::Weights4"));
             AbstractDataTypePtr y(new const annot::PiecesADT<hip::MatvecOut>("y", "gernels::MatvecOut", "at", {{"columns", &hip::MatvecOut::columns}}));
-            annot::PieceFunction multiply("gernels::multiply_4bit", "gernels/matvec4.h", {x, weights}, y, {"columns"},
+            annot::PieceFunction multiply("gernels::multiply_4bit", "gernels/serving/matvec4.h", {x, weights}, y, {"columns"},
                                           {"group", "row_tiles", "column_tiles", "waves"});
             Variable column("column"), threads("threads");
             Composable program =

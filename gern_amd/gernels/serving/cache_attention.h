@@ -1,4 +1,4 @@
-// Attention of queries over a paged 8-bit cache (gernels/paged_cache.h).
+// Attention of queries over a paged 8-bit cache (gernels/serving/paged_cache.h).
 //
 // Request r has n queries (consecutive tokens) and holds `length` keys; with
 // G query heads to a head of the cache, query i of head h' = h G + u sees the
@@ -38,8 +38,8 @@
 // moves 5.2 on the same GPU).
 #pragma once
 
-#include "gernels/half_tiles.h"
-#include "gernels/paged_cache.h"
+#include "gernels/serving/half_tiles.h"
+#include "gernels/serving/paged_cache.h"
 
 namespace gernels {
 

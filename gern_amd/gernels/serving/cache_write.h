@@ -1,4 +1,4 @@
-// New keys and values into a paged cache (gernels/paged_cache.h).
+// New keys and values into a paged cache (gernels/serving/paged_cache.h).
 //
 // Token t goes to slot[t] = page * P + place (-1: nowhere).  For every page and
 // head, over what the page holds in front of the new tokens and what is added:
@@ -23,8 +23,8 @@
 // heads of 128 in 5.1 us.
 #pragma once
 
-#include "gernels/half_tiles.h"
-#include "gernels/paged_cache.h"
+#include "gernels/serving/half_tiles.h"
+#include "gernels/serving/paged_cache.h"
 
 namespace gernels {
 

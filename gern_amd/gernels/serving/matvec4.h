@@ -27,7 +27,7 @@
 // ALU, which takes 7 instructions for 8 codes and 8 for the sums of a group).
 #pragma once
 
-#include "gernels/half_tiles.h"
+#include "gernels/serving/half_tiles.h"
 
 namespace gernels {
 

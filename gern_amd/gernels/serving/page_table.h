@@ -19,7 +19,7 @@
 // writing.
 #pragma once
 
-#include "gernels/paged_cache.h"
+#include "gernels/serving/paged_cache.h"
 
 namespace gernels {
 
