@@ -182,7 +182,8 @@ int gern_qk_softmax_run_no_alloc(gern_pipeline p, const uint16_t *Q, const uint1
  * The cache: a page holds page_size (16, 32, 64 or 128) consecutive tokens of
  * one request.  Codes are [pages, heads, page_size, head_dim] bytes in e4m3
  * (4 exponent bits, 3 mantissa bits, +-448, no infinities), scales [pages,
- * heads] fp32, both for keys and for values; a value is code * scale.
+ * heads] fp32, not negative, both for keys and for values; a value is code *
+ * scale.
  * pages * page_size is less than 2^31.  A slot is page * page_size + place.
  * head_dim is 64, 128, 192 or 256.
  *
@@ -243,7 +244,8 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  * the cache.
  *   O = softmax(scale * q . k) v over the keys a query sees, 0 where it sees none
  * (a request of length 0, a query in front of the first key), in `type`, row
- * stride ldo; rows of Q in no request are left alone in O.
+ * stride ldo; rows of Q in no request are left alone in O.  O may be Q (with the
+ * same stride); it shares memory with nothing else that the call reads.
  * max_queries and max_length tell the most queries and keys of one request; the
  * division of the work and the workspace depend on them and the results do not
  * (more are computed, too, only slower).  The workspace

@@ -38,6 +38,7 @@ def i32(torch, a):
 
 def run_tables(torch, gpu, cached, added, page, width, count, tokens, seed=0, capacity=None):
     rs = np.random.RandomState(seed)
+    cached, added = (np.asarray(a, dtype=np.int64) for a in (cached, added))
     n = len(cached)
     held = -(-np.maximum(cached, 0) // page)
     order = rs.permutation(int(held.sum()) + max(count, capacity or 0))
@@ -65,7 +66,7 @@ def test_tables(torch, gpu, n, page):
     run_tables(torch, gpu, cached, added, page, width=8, count=8 * n + 3, tokens=int(added.sum()) + n % 3, seed=n)
 
 
-@pytest.mark.parametrize("cached, added", [([0], [0]), ([0], [1]), ([16], [1]), ([15], [1]), ([15], [2]), ([0, 0, 0], [0, 0, 0]), ([5, 0, 7], [0, 40, 0]),
+@pytest.mark.parametrize("cached, added", [([], []), ([0], [0]), ([0], [1]), ([16], [1]), ([15], [1]), ([15], [2]), ([0, 0, 0], [0, 0, 0]), ([5, 0, 7], [0, 40, 0]),
                                            ([-3, 4], [2, -5]), ([1], [100_000])])
 def test_tables_of_few_requests(torch, gpu, cached, added):
     cached, added = np.array(cached), np.array(added)
@@ -450,6 +451,21 @@ def test_matvec_row_with_nan_stays_alone(torch, gpu):
     gpu("Matvec4", group=128, dtype="bf16")(x[:0], codes, scales, y[:0])
 
 
+def test_matvec_codes_beyond_32_bits(torch, gpu):
+    """5.2 GB of codes: the last columns, whose rows begin behind 2^32 bytes."""
+    n, k, group = 40000, 262144, 128
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x = torch.randn((2, k), generator=g, device="cuda").bfloat16()
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((k // group, n), generator=g, device="cuda") * 0.01 + 0.005).bfloat16()
+    y = torch.zeros((2, n), dtype=torch.bfloat16, device="cuda")
+    gpu("Matvec4", group=group, dtype="bf16")(x, codes, scales, y)
+    for at in (slice(0, 4), slice(n - 4, n)):
+        want, tol = so.matvec4(x.double().cpu().numpy(), codes[at].cpu().numpy(), scales[:, at].double().cpu().numpy(), np.full((k // group, 4), 8.0), group, 128)
+        assert np.all(np.abs(y[:, at].double().cpu().numpy() - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol))
+
+
 # ------------------------------------------------------------------------------------------------ a step
 
 
@@ -547,6 +563,44 @@ def test_a_serving_step(torch, gpu):
                     assert np.all(np.abs(got[starts[b]:starts[b + 1], u] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol)), (turn, b, u)
         state["cached"].copy_(state["lengths"])
         state["count"].copy_(state["counts"][:1])
+
+
+@pytest.mark.parametrize("queries", [1, 100])
+def test_cache_beyond_32_bits(torch, gpu, queries):
+    """Pages behind 2^32 bytes of codes: the same bits as from a small cache, and pages in front of them are left alone."""
+    dim, page, heads, tokens, pages = 256, 128, 1, 300, 140_000
+    assert pages * heads * page * dim > 2 ** 32
+    rs = np.random.RandomState(30)
+    write, attend = gpu("CacheWrite", head_dim=dim, page_size=page, dtype="bf16"), gpu("CacheAttention", head_dim=dim, page_size=page, dtype="bf16")
+    k, v = (torch.from_numpy(rs.normal(size=(tokens, heads, dim))).bfloat16().cuda() for _ in range(2))
+    q = torch.from_numpy(rs.normal(size=(queries, 4, dim))).bfloat16().cuda()
+    results = []
+    for total, held in ((4, [0, 3, 1]), (pages, [pages - 1, pages - 3, 7])):
+        kc, vc = (torch.zeros((total, heads, page, dim), dtype=torch.uint8, device="cuda") for _ in range(2))
+        ks, vs = (torch.ones((total, heads), device="cuda") for _ in range(2))
+        slots = np.array(held).repeat(page)[:tokens] * page + np.arange(tokens) % page
+        write(k, v, i32(torch, slots), kc, vc, ks, vs)
+        out = torch.zeros_like(q)
+        attend(q, kc, vc, ks, vs, i32(torch, [held]), i32(torch, [tokens]), i32(torch, [0, queries]), out, 0.06, max_queries=queries)
+        torch.cuda.synchronize()
+        assert write.faults() == 0 and attend.faults() == 0
+        assert int(kc.view(torch.int64).count_nonzero()) <= 3 * page * dim // 8
+        results.append((out.clone(), kc[held].clone(), vc[held].clone(), ks[held].clone()))
+        del kc, vc
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_attention_in_place(torch, gpu):
+    """The result may take the queries' place."""
+    for queries in (1, 60):
+        device, host, out = attention_inputs(torch, "bf16", 128, 32, 2, 4, [700, 90], [queries, 2], seed=31)
+        a = gpu("CacheAttention", head_dim=128, page_size=32, dtype="bf16")
+        a(**device, scale=0.1, max_queries=queries, max_length=700)
+        device["out"] = device["q"]
+        a(**device, scale=0.1, max_queries=queries, max_length=700)
+        torch.cuda.synchronize()
+        n = int(host["starts"][-1])
+        assert torch.equal(device["q"][:n], out[:n, :8])
 
 
 def test_two_streams_at_a_time(torch, gpu):
