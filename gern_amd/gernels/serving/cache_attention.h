@@ -242,14 +242,16 @@ struct RowState {
         }
     }
 
-    // Adds the keys [base, base + 32): fragment i of 16-key tile t is key_frag(t, i), of V^T value_frag(i).
-    // `whole`: every row sees all of them.  after_keys() is called when the keys' fragments have been used.
-    template<class KeyFrag, class AfterKeys, class Scales, class ValueFrag>
+    // Adds the keys [base, base + 32 PAIRS): fragment i of 16-key tile t is key_frag(t, i), of V^T of the p-th pair of
+    // tiles value_frag(p, i).  `whole`: every row sees all of them.  after_keys() is called when the keys' fragments have
+    // been used.
+    template<int PAIRS, class KeyFrag, class Scales, class AfterKeys, class ValueFrag>
     __device__ __forceinline__ void add(int base, bool whole, KeyFrag key_frag, Scales scales_of_tile, AfterKeys after_keys, ValueFrag value_frag) {
+        constexpr int kTiles = 2 * PAIRS;
         const int g = lane_id() / 16;
-        f32x4 s[R][2];
+        f32x4 s[R][kTiles];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < kTiles; t++) {
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 s[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -263,24 +265,32 @@ struct RowState {
                 }
             }
         }
-        const TileScales scales[2] = {scales_of_tile(0), scales_of_tile(1)};
+        TileScales scales[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) {
+            scales[t] = scales_of_tile(t);
+        }
         after_keys();
-        Frag p[R];
+        Frag p[R][PAIRS];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if (!whole) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool seen = scales[j / 4].there && base + 16 * (j / 4) + 4 * g + j % 4 < limit[r];
-                    s[r][j / 4][j % 4] = seen ? s[r][j / 4][j % 4] : -__builtin_inff();
+                for (int t = 0; t < kTiles; t++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool seen = scales[t].there && base + 16 * t + 4 * g + e < limit[r];
+                        s[r][t][e] = seen ? s[r][t][e] : -__builtin_inff();
+                    }
                 }
             }
             // scales are not negative: the largest product of a tile is its largest score
             float top = kLowest;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < kTiles; t++) {
                 const float most = larger(larger(s[r][t][0], s[r][t][1]), larger(s[r][t][2], s[r][t][3]));
-                top = larger(top, __builtin_fmaf(most, scales[t].k, scales[t].up));
+                const float score = __builtin_fmaf(most, scales[t].k, scales[t].up);
+                top = t == 0 ? score : larger(top, score);
             }
             top = max_over_lane_groups(top);
             if (__ballot(top > m[r]) != 0) {
@@ -293,27 +303,28 @@ struct RowState {
                     o[r][i] *= shrink;
                 }
             }
-            float y[8];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < kTiles; t++) {
                 const float shift = scales[t].up - m[r];
+                float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    y[4 * t + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][e], scales[t].k, shift));
-                    l[r] = __builtin_fmaf(y[4 * t + e], scales[t].per_v, l[r]);
+                    y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][e], scales[t].k, shift));
+                    l[r] = __builtin_fmaf(y[e], scales[t].per_v, l[r]);
                 }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                p[r].w[j] = pack_halves<F16>(y[2 * j], y[2 * j + 1]);
+                p[r][t / 2].w[2 * (t % 2)] = pack_halves<F16>(y[0], y[1]);
+                p[r][t / 2].w[2 * (t % 2) + 1] = pack_halves<F16>(y[2], y[3]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-            const Frag v = value_frag(i);
+        for (int pair = 0; pair < PAIRS; pair++) {
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                o[r][i] = mfma_16x16x32<false>(v, p[r], o[r][i]);
+            for (int i = 0; i < D / 16; i++) {
+                const Frag v = value_frag(pair, i);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    o[r][i] = mfma_16x16x32<false>(v, p[r][pair], o[r][i]);
+                }
             }
         }
     }
@@ -458,7 +469,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
             const bool whole = base + 32 <= least && there[0] && there[1];
             missing = missing || !there[0] || (!there[1] && base + 16 < end);
             const bool more = base + kStep < end;
-            state.add(
+            state.template add<1>(
                 base, whole, [&](int t, int i) { return keys[t].template key_frag<T::kBf16>(i); },
                 [&](int t) { return detail::scales_of(keys[t], __builtin_fabsf(batch.scale)); },
                 [&]() {
@@ -473,7 +484,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
                         id[1] = walk.look_up(base + 2 * kStep + 16);
                     }
                 },
-                [&](int i) {
+                [&](int, int i) {
                     const Words2 a = keys[0].value_half(i), b = keys[1].value_half(i);
                     return detail::Frag{{a.w[0], a.w[1], b.w[0], b.w[1]}};
                 });
@@ -628,32 +639,30 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
                 id = walk.look_up(base + 2 * kBlock + 16 * wave);
                 walk.load_values(keys, base + kBlock + 16 * wave);
             }
+            if (base < min(most, end)) {
+                detail::TileScales scales[WAVES];
+                bool there = true;
 #pragma unroll
-            for (int pair = 0; pair < WAVES / 2; pair++) {
-                const int at = base + 32 * pair;
-                if (at < min(most, end)) {
-                    detail::TileScales scales[2];
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        uint32_t x[4];
-                        detail::load_words<4>(x, reinterpret_cast<const uint32_t *>(tile_scales[buffer][2 * pair + t]));
-                        scales[t] = {as_float((int)x[0]), as_float((int)x[1]), as_float((int)x[2]), __builtin_amdgcn_readfirstlane((int)x[3]) != 0};
-                    }
-                    const bool whole = at + 32 <= least && scales[0].there && scales[1].there;
-                    state.add(
-                        at, whole,
-                        [&](int t, int i) {
-                            detail::Frag k;
-                            detail::load_words<4>(k.w, k_frags[buffer][2 * pair + t][i][lane]);
-                            return k;
-                        },
-                        [&](int t) { return scales[t]; }, [] {},
-                        [&](int i) {
-                            detail::Frag v;
-                            detail::load_words<4>(v.w, v_frags[buffer][pair][i][lane]);
-                            return v;
-                        });
+                for (int t = 0; t < WAVES; t++) {
+                    uint32_t x[4];
+                    detail::load_words<4>(x, reinterpret_cast<const uint32_t *>(tile_scales[buffer][t]));
+                    scales[t] = {as_float((int)x[0]), as_float((int)x[1]), as_float((int)x[2]), __builtin_amdgcn_readfirstlane((int)x[3]) != 0};
+                    there = there && scales[t].there;
                 }
+                // the whole block at once: fewer lane exchanges a key
+                state.template add<WAVES / 2>(
+                    base, base + kBlock <= least && there,
+                    [&](int t, int i) {
+                        detail::Frag k;
+                        detail::load_words<4>(k.w, k_frags[buffer][t][i][lane]);
+                        return k;
+                    },
+                    [&](int t) { return scales[t]; }, [] {},
+                    [&](int pair, int i) {
+                        detail::Frag v;
+                        detail::load_words<4>(v.w, v_frags[buffer][pair][i][lane]);
+                        return v;
+                    });
             }
             if (kBuffers == 1) {
                 __syncthreads();  // this block has been read
