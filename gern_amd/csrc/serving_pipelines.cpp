@@ -336,9 +336,14 @@ struct AttentionPlan {
 
 constexpr int64_t kMaxSplits = 256;  // gernels/serving/cache_attention.h, join_splits
 
-// The programs of a pipeline, four wavefronts a workgroup: few rows (queries times the heads that share a head of the
-// cache) against keys that the wavefronts divide, or many rows divided among the wavefronts.
-constexpr int64_t kAttentionWaves = 4;
+// The programs of a pipeline: few rows (queries times the heads that share a head of the cache) against keys that the
+// wavefronts divide, many rows divided among the wavefronts, and few rows on twice the wavefronts where workgroups are few.
+struct AttentionProgram {
+    bool few;
+    int64_t waves;
+};
+constexpr AttentionProgram kAttentionPrograms[] = {{true, 4}, {false, 4}, {true, 8}};
+constexpr size_t kFewRows = 0, kManyRows = 1, kFewRowsWide = 2, kJoinWave = 3, kJoinWorkgroup = 4;
 
 // 16-row tiles of a wavefront of the second: accumulators and queries take 3/8 R D registers a lane, and two
 // wavefronts are to fit a SIMD.
@@ -355,8 +360,8 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     AttentionPlan plan{};
     // 32 requests of 2000 to 4000 keys, 8 heads of 128, us with few / many rows a program: 16 rows 56 / 91, 32 rows 63 / 93,
     // 64 rows 91 / 101.
-    plan.variant = rows <= 64 ? 0 : 1;
-    const int64_t tile = plan.variant == 0 ? 16 : 16 * kAttentionWaves * attentionRowTiles(head_dim);
+    plan.variant = rows <= 64 ? kFewRows : kManyRows;
+    const int64_t tile = plan.variant == kFewRows ? 16 : 16 * kAttentionPrograms[kManyRows].waves * attentionRowTiles(head_dim);
     plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
     // Keys are split, into pieces of at least 512, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
     // to three times what is resident, so that requests of different lengths leave few CUs idle at the end.  Few rows of
@@ -364,13 +369,19 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     // Measured (us) with 512 / 1024 / 2048 / 4096: 64 requests of 4096 to 8192 keys, 8 heads of 128: 181 / 175 / 155 /
     // 165; 3 of 131072 to 262144: 266 / 188 / 184 / 197; 32 of 1250 to 2500, 16 heads of 256: 95 / 110 / 109 / -; 6 of 113
     // to 447 queries and 4032 to 5915 keys, 4 heads of 64 for 16: - / 103 / 97 / 103.
-    const int64_t wanted = plan.variant == 0 && head_dim > 128 ? 512 : 2048;
+    const int64_t wanted = plan.variant == kFewRows && head_dim > 128 ? 512 : 2048;
     const int64_t whole = requests * heads * plan.row_tiles;
-    // Up to 1024 keys are not worth a second launch (1 request of 700, 8 heads of 128: 10.4 us whole, 13.9 split; 1000:
-    // 12.3, 11.9; 2000: 18.6, 13.4), nor are workgroups for every CU four times over (128 requests of 1000 to 2000, 8 heads
+    // Up to 1024 keys are not worth a second launch (1 request of 1000, 8 heads of 128: 10.3 us whole, 11.9 split;
+    // 2000: 16.0, 12.1), nor are workgroups for every CU four times over (128 requests of 1000 to 2000, 8 heads
     // of 128: 87 whole, 97 in two).  Pieces of 256 / 512 / 1024 at least: 16 requests of 2000 to 4000 33.3 / 31.7 / 27.5, one
     // of 32768 18.4 / 17.1 / 19.5, two of 20000, 4 heads 16.0 / 15.8 / 18.6.
     const int64_t splits = max_length <= 1024 || whole >= 1024 ? 1 : std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
+    // Undivided keys, and a CU for every workgroup: its wavefronts' steps of 32 keys one after the other are what a call
+    // takes, so there are twice as many.  8 heads of 128, us with 4 / 8 wavefronts: 1 request of 1000 keys 11.3 / 10.3, 32 of
+    // 1000 15.1 / 13.7 (of 256: 23.6 / 23.8); 1 of 500 9.4 / 9.5 (of 256: 10.1 / 10.4); 64 of 1000, two workgroups a CU, 24 / 26.
+    if (plan.variant == kFewRows && max_length > 512 && max_length <= 1024 && whole <= 256) {
+        plan.variant = kFewRowsWide;
+    }
     plan.chunk = std::max<int64_t>(512, ((max_length + splits - 1) / splits + 255) / 256 * 256);
     plan.splits = std::max<int64_t>(1, (max_length + plan.chunk - 1) / plan.chunk);
     // BLOCK_Y holds 65535 pieces; a workgroup takes further row tiles in turn
@@ -417,7 +428,8 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
         const std::string header = "gernels/serving/cache_attention.h", batch_type = "gernels::AttentionBatchOf<" + typeName(type) + ">";
         AbstractDataTypePtr batch(new const annot::WholeADT("batch", batch_type));
         AbstractDataTypePtr cache(new const annot::WholeADT("cache", "gernels::PagedCache"));
-        for (bool few : {true, false}) {
+        for (const AttentionProgram &attention : kAttentionPrograms) {
+            const bool few = attention.few;
             using Out = hip::AttentionOut;
             AbstractDataTypePtr result(new const annot::PiecesADT<Out>("result", "gernels::AttentionOut", "piece",
                                                                       {{"pieces", &Out::pieces}, {"heads", &Out::heads}, {"requests", &Out::requests}}));
@@ -425,7 +437,7 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
                                                              std::vector<std::string>{"head_dim", "page", "row_tiles", "waves"};
             annot::PieceFunction attend(few ? "gernels::attend_few_rows" : "gernels::attend_many_rows", header, {batch, cache}, result,
                                         {"pieces", "heads", "requests"}, constants);
-            std::map<std::string, Variable> bound{constant("head_dim", head_dim), constant("page", page_size), constant("waves", kAttentionWaves)};
+            std::map<std::string, Variable> bound{constant("head_dim", head_dim), constant("page", page_size), constant("waves", attention.waves)};
             if (!few) {
                 bound.insert(constant("row_tiles", attentionRowTiles(head_dim)));
             }
@@ -435,7 +447,7 @@ int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, i
             Composable program = Global(
                 (Tile(result["pieces"], x.bind(1)) || Grid::BLOCK_Y)((Tile(result["heads"], head.bind(1)) || Grid::BLOCK_X)(
                     (Tile(result["requests"], request.bind(1)) || Grid::BLOCK_Z)(attend[bound](batch, cache, result)))),
-                {{Grid::BLOCK_DIM_X, threads.bind(64 * kAttentionWaves)}});
+                {{Grid::BLOCK_DIM_X, threads.bind(64 * attention.waves)}});
             // wavefronts of the second program on a SIMD
             if (p.add(program, flags | GERN_PIPELINE_NO_XCD_REMAP, few ? attentionResidentWaves(head_dim) : head_dim == 64 ? 3 : 2) != 0) {
                 return 1;
@@ -531,7 +543,7 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     }
     const bool wave_a_row = plan.splits <= 16;
     hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, wave_a_row ? (rows + 3) / 4 : rows};
-    const int joined = evaluate(p, wave_a_row ? 2 : 3, who, stream, {{"batch", &batch}, {"rows", &join}});
+    const int joined = evaluate(p, wave_a_row ? kJoinWave : kJoinWorkgroup, who, stream, {{"batch", &batch}, {"rows", &join}});
     p->last_variant = plan.variant;
     return joined;
 }

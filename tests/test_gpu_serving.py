@@ -321,6 +321,12 @@ def test_attention_several_queries(torch, gpu, dtype, dim, page, group):
     run_attention(torch, gpu, dtype, dim, page, 2, group, [0, 0, 9, 300, 150, 200, 64], [0, 2, 20, 130, 150, 1, 0], seed=2)
 
 
+@pytest.mark.parametrize("dtype, dim, page, group", [("f16", 64, 16, 4), ("bf16", 128, 32, 3), ("bf16", 192, 16, 20), ("f16", 256, 64, 1)])
+def test_attention_of_up_to_1024_keys(torch, gpu, dtype, dim, page, group):
+    """A call of few workgroups whose keys eight wavefronts divide: lengths at the ends of their steps of 256 keys, several rows."""
+    run_attention(torch, gpu, dtype, dim, page, 2, group, [1024, 513, 0, 1, 255, 256, 257, 1000, 33], [1, 3, 1, 2, 1, 1, 2, 3, 0], seed=dim)
+
+
 def test_attention_rows_that_see_nothing(torch, gpu):
     for queries in (1, 100):
         device, host, out = attention_inputs(torch, "bf16", 128, 16, 1, 4, [0, 1], [queries, queries], seed=4)
