@@ -163,6 +163,20 @@ struct RawKeys {
             }
         }
     }
+    // Makes 0 of the values that are NaN (codes 127 and 255); whether there were any.
+    __device__ __forceinline__ bool take_nan() {
+        uint32_t found = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int w = 0; w < D / 64; w++) {
+                const uint32_t nan = ((v[j][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                v[j][w] &= ~((nan >> 7) * 0xffu);
+                found |= nan;
+            }
+        }
+        return __ballot(found != 0) != 0;
+    }
 };
 
 // The scales of a tile as the softmax takes them.
@@ -399,7 +413,44 @@ struct AttentionRequest {
     __device__ __forceinline__ int64_t part(int row, const AttentionPiece &piece) const {
         return split * all_rows + token(row) * (piece.to.heads * group) + head(row, piece);
     }
+    // Where a dimension of a row's result, or of its part, is; set to NaN.
+    __device__ __forceinline__ void put_nan(int row, int d, const AttentionPiece &piece) const {
+        if (splits == 1) {
+            reinterpret_cast<unsigned short *>(piece.to.out + token(row) * piece.to.out_pitch + head(row, piece) * (D / 2))[d] = 0x7fff;
+        } else {
+            piece.to.partial[part(row, piece) * D + d] = __builtin_nanf("");
+        }
+    }
 };
+
+// NaN among the values of keys that some rows of a workgroup see and others do not is taken out (0 * NaN must not reach a
+// row that does not see the key) and put into the results of the rows that do when they are stored.  This does so for the
+// 16 keys at `base` and the rows [row, end).  It is rare, and reads the codes again: kept from the loop over the keys,
+// whatever would be noted there costs every call (64 requests: 162 to 177 us for 155).
+template<int D, int PAGE, class T>
+__device__ __forceinline__ void return_nan(AttentionRequest<D, PAGE, T> request, const AttentionPiece &piece, const KeyWalk<D, PAGE> &walk, int base,
+                                           int row, int end) {
+    // what this computes is not to be held in registers from before the loop over the keys
+    asm volatile("" : "+s"(request.group), "+s"(request.first), "+s"(request.splits));
+    const int lane = lane_id() + opaque_zero(), key = lane / 4, quarter = lane % 4;
+    const int id = walk.look_up(base);
+    if (id < 0 || id >= walk.cache.pages || base >= walk.length) {
+        return;
+    }
+    const uint32_t *v = walk.cache.v + ((int64_t)id * walk.cache.heads + walk.head) * (PAGE * D / 4);
+    const unsigned char *codes = reinterpret_cast<const unsigned char *>(v) + (base % PAGE + key) * D;
+#pragma unroll 1
+    for (int d = quarter * (D / 4); d < (quarter + 1) * (D / 4); d++) {
+        if ((codes[d] & 127) == 127) {
+#pragma unroll 1
+            for (int r = row; r < end; r++) {
+                if (base + key < request.limit(r)) {
+                    request.put_nan(r, d, piece);
+                }
+            }
+        }
+    }
+}
 
 // Queries and limits of the R tiles of rows from row0 on.
 template<int D, int PAGE, int R, class T>
@@ -450,10 +501,11 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         // `end` cuts a tile only where no row sees further: splits are whole tiles
         const int end = request.split + 1 < request.splits ? (int)min(begin + to.chunk, (int64_t)most) : most;
         constexpr int kStep = 32 * WAVES;
-        bool missing = false;
+        bool missing = false, nan = false;
         // Keys of the next step are loaded when this step's have been multiplied, values likewise, page numbers a step
         // before: no register is held for a load that waits, and none of the loads is waited for where it is issued.
-        int base = (int)min(begin, (int64_t)most) + 32 * wave;
+        const int first = (int)min(begin, (int64_t)most) + 32 * wave;
+        int base = first;
         detail::RawKeys<D> keys[2];
         int id[2] = {walk.look_up(base), walk.look_up(base + 16)};
         if (base < end) {
@@ -476,6 +528,8 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
                     if (!whole) {
                         keys[0].clear_values_behind(base, request.length);
                         keys[1].clear_values_behind(base + 16, request.length);
+                        nan = keys[0].take_nan() || nan;
+                        nan = keys[1].take_nan() || nan;
                     }
                     if (more) {
                         walk.load_keys(keys[0], base + kStep, id[0]);
@@ -504,6 +558,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         constexpr int kPart = D / 16;
         __shared__ __attribute__((aligned(16))) float parts[WAVES][16][kPitch];
         __shared__ float part_m[WAVES][16], part_l[WAVES][16];
+        __shared__ int part_nan[WAVES];
         static_assert(WAVES >= 4, "256 threads share 16 rows");
         __syncthreads();  // the previous rows have been read
 #pragma unroll
@@ -517,6 +572,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         if (g == 0) {
             part_m[wave][c] = state.m[0];
             part_l[wave][c] = state.l[0];
+            part_nan[wave] = nan;
         }
         __syncthreads();
         const int at = threadIdx.x / 16, d = (threadIdx.x % 16) * kPart, row = row0 + at;
@@ -556,6 +612,20 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
                 }
             }
         }
+        int any_nan = part_nan[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            any_nan |= part_nan[w];
+        }
+        if (__builtin_amdgcn_readfirstlane(any_nan) != 0) {
+            __syncthreads();  // the results are stored
+            for (int at = first; nan && at < end; at += kStep) {
+                // (a tile was not whole either where its neighbour's page is missing)
+                for (int t = 0; t < 2 && (missing || at + 32 > least); t++) {
+                    detail::return_nan(request, piece, walk, at + 16 * t, row0, min(request.rows, row0 + 16));
+                }
+            }
+        }
     }
 }
 
@@ -584,26 +654,28 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
     constexpr int kBuffers = D <= 128 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) uint32_t k_frags[kBuffers][WAVES][D / 32][kWaveSize][4];
     __shared__ __attribute__((aligned(16))) uint32_t v_frags[kBuffers][WAVES / 2][D / 16][kWaveSize][4];
-    __shared__ __attribute__((aligned(16))) float tile_scales[kBuffers][WAVES][4];  // k, up, per_v, there
+    __shared__ __attribute__((aligned(16))) float tile_scales[kBuffers][WAVES][4];  // k, up, per_v, 1 there | 2 NaN taken
 
     for (int tile = (int)piece.x / request.splits; tile * kTileRows < request.rows; tile += tiles) {
         const int row0 = tile * kTileRows + wave * kRows;
         detail::RowState<D, R, T::kBf16> state;
         state.clear();
         detail::load_queries(state, request, batch, piece, row0);
-        // keys that any row of the workgroup, and any / every row of this wavefront sees
-        const int all = request.limit(min((tile + 1) * kTileRows, request.rows) - 1);
+        // keys that any / every row of the workgroup, and any / every row of this wavefront sees
+        const int all = request.limit(min((tile + 1) * kTileRows, request.rows) - 1), least_of_all = request.limit(tile * kTileRows);
         const int most = row0 < request.rows ? request.limit(min(row0 + kRows, request.rows) - 1) : 0;
         const int least = row0 < request.rows ? request.limit(row0) : 0;
         const int64_t begin64 = (int64_t)request.split * to.chunk;
         const int begin = (int)min(begin64, (int64_t)all);
         const int end = request.split + 1 < request.splits ? (int)min(begin64 + to.chunk, (int64_t)all) : all;
-        bool missing = false;
+        bool missing = false, nan = false;
 
         detail::RawKeys<D> keys;
         auto stage = [&](int buffer, int base) {
-            if (!keys.there || base + 16 > request.length) {
+            bool taken = false;
+            if (!keys.there || base + 16 > least_of_all) {
                 keys.clear_values_behind(base, request.length);
+                taken = keys.take_nan();
             }
 #pragma unroll
             for (int i = 0; i < D / 32; i++) {
@@ -616,7 +688,7 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
             }
             const detail::TileScales scales = detail::scales_of(keys, scale);
             if (lane == 0) {
-                const float x[4] = {scales.k, scales.up, scales.per_v, scales.there ? 1.0f : 0.0f};
+                const float x[4] = {scales.k, scales.up, scales.per_v, as_float((scales.there ? 1 : 0) | (taken ? 2 : 0))};
                 detail::store_floats(tile_scales[buffer][wave], x);
             }
             missing = missing || (!keys.there && base < end);
@@ -646,8 +718,11 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
                 for (int t = 0; t < WAVES; t++) {
                     uint32_t x[4];
                     detail::load_words<4>(x, reinterpret_cast<const uint32_t *>(tile_scales[buffer][t]));
-                    scales[t] = {as_float((int)x[0]), as_float((int)x[1]), as_float((int)x[2]), __builtin_amdgcn_readfirstlane((int)x[3]) != 0};
+                    scales[t] = {as_float((int)x[0]), as_float((int)x[1]), as_float((int)x[2]), false};
+                    const int flags = __builtin_amdgcn_readfirstlane((int)x[3]);
+                    scales[t].there = (flags & 1) != 0;
                     there = there && scales[t].there;
+                    nan = nan || (flags & 2) != 0;
                 }
                 // the whole block at once: fewer lane exchanges a key
                 state.template add<WAVES / 2>(
@@ -701,6 +776,14 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
                 if (request.splits > 1 && g == 0) {
                     to.stats[2 * part] = state.m[r];
                     to.stats[2 * part + 1] = sum;
+                }
+            }
+        }
+        if (nan) {
+            __threadfence_block();  // this wavefront's results are stored
+            for (int at = begin; at < min(most, end); at += 16) {
+                if (at + 16 > least_of_all) {
+                    detail::return_nan(request, piece, walk, at, row0, min(request.rows, row0 + kRows));
                 }
             }
         }

@@ -395,6 +395,49 @@ def test_attention_leaves_out_pages_outside_the_cache(torch, gpu, queries):
                 assert np.all(np.abs(o[i, u] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol))
 
 
+@pytest.mark.parametrize("dim, page, group", [(64, 16, 3), (128, 32, 1), (192, 64, 2), (256, 16, 2)])
+@pytest.mark.parametrize("length, queries", [(90, 3), (90, 90), (700, 20), (1300, 300), (9000, 6)])
+def test_attention_nan_stays_with_the_queries_that_see_it(torch, gpu, dim, page, group, length, queries):
+    """NaN among the values, and among the keys, of tokens that the first queries do not see."""
+    device, host, out = attention_inputs(torch, "bf16", dim, page, 1, group, [length, 50], [queries, 50], seed=length + dim)
+    rs = np.random.RandomState(length)
+    odd = np.zeros((length, dim), dtype=bool)
+    for key in {length - 1, length - 2, length - 1 - queries // 2}:
+        for d in (0, dim - 1, rs.randint(dim)):
+            odd[key, d] = True
+    codes = device["v_cache"].cpu().numpy()
+    pages = host["table"][0, :-(-length // page)]
+    for key, d in zip(*np.nonzero(odd)):
+        codes[pages[key // page], 0, key % page, d] = rs.choice([127, 255])
+    device["v_cache"] = torch.from_numpy(codes).cuda()
+    a = gpu("CacheAttention", head_dim=dim, page_size=page, dtype="bf16")
+    ws = torch.empty(a.workspace_bytes(device["q"].shape[0], 2, group, 1, max(queries, 50), length), dtype=torch.uint8, device="cuda")
+    o = {}
+    for blind in (False, True):
+        if blind:  # the last token's key as well: the last query is NaN throughout
+            device["k_cache"][int(pages[-1]), 0, (length - 1) % page, dim // 3] = 127
+        a(**device, scale=0.09, max_queries=max(queries, 50), max_length=length, workspace=ws)
+        torch.cuda.synchronize()
+        assert a.faults() == 0
+        o[blind] = out.double().cpu().numpy()
+    for r, n in enumerate(host["lengths"]):
+        at, m = host["starts"][r], host["starts"][r + 1] - host["starts"][r]
+        mine = host["table"][r, :-(-n // page)]
+        k, v = ((host["codes"][s][mine, 0] * host["scales"][s][mine, 0][:, None, None]).reshape(-1, dim)[:n] for s in (0, 1))
+        vs = np.repeat(host["scales"][1][mine, 0], page)[:n]
+        seen = n - m + np.arange(m) + 1
+        nan = np.array([odd[:max(c, 0)].any(axis=0) for c in seen]) if r == 0 else np.zeros((m, dim), dtype=bool)
+        for u in range(group):
+            want, tol = so.attention(host["q"][at:at + m, u], k, np.where(odd, 0.0, v) if r == 0 else v, vs, seen, 0.09)
+            tol = tol + HALF_STEP["bf16"] * (np.abs(want) + tol)
+            for blind in (False, True):
+                got, expect = o[blind][at:at + m, u], nan.copy()
+                if blind and r == 0:
+                    expect[m - 1] = True
+                assert np.array_equal(np.isnan(got), expect), (r, u, blind)
+                assert np.all(np.abs(got - want)[~expect] <= np.broadcast_to(tol, want.shape)[~expect])
+
+
 def test_attention_length_beyond_the_table(torch, gpu):
     device, host, out = attention_inputs(torch, "bf16", 64, 16, 1, 1, [64, 20], [1, 1], seed=9)
     device["table"] = device["table"][:, :4].contiguous()
