@@ -107,6 +107,11 @@ bool aligned(const void *pointer, uintptr_t bytes) {
     return reinterpret_cast<uintptr_t>(pointer) % bytes == 0;
 }
 
+// A launch has less than 2^32 threads along x.
+bool tooWide(int64_t workgroups, int64_t threads) {
+    return workgroups * threads > 0xffffffff;
+}
+
 // Whether [a, a + na) and [b, b + nb), sizes in bytes, share memory.
 bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
     const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
@@ -320,6 +325,9 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
     if (pieces > 0x7fffffff) {
         return fail("gern_cache_write_run: tokens / page_size * heads must be less than 2^30");
     }
+    if (tooWide(pieces, single ? 64 : 256)) {
+        return fail("gern_cache_write_run: tokens / page_size * heads must be less than 2^23");
+    }
     hip::WritableCache cache{{k_cache, v_cache, k_scales, v_scales, pages, heads, p->fault_count}, pieces, stretch};
     return evaluate(p, single ? 0 : 1, "gern_cache_write_run", stream, {{"tokens", &fresh}, {"cache", &cache}});
 }
@@ -528,10 +536,14 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
         return fail("gern_cache_attention_run: the workspace must be 16-byte aligned and hold the " + std::to_string(needed) +
                     " bytes that gern_cache_attention_workspace says");
     }
+    const bool wave_a_row = plan.splits <= 16;
+    const int64_t rows = tokens * q_heads, join_blocks = wave_a_row ? (rows + 3) / 4 : rows;
+    if (needed > 0 && tooWide(join_blocks, 256)) {
+        return fail("gern_cache_attention_run: tokens * q_heads must be less than 2^24 where keys are split into more than 16 pieces, 2^26 into fewer");
+    }
     if (needed > 0 && overlap(workspace, needed, O, ((tokens - 1) * ldo + q_heads * p->head_dim) * 2)) {
         return fail("gern_cache_attention_run: the workspace shares memory with O");
     }
-    const int64_t rows = tokens * q_heads;
     float *partial = static_cast<float *>(workspace), *stats = needed > 0 ? partial + plan.splits * rows * p->head_dim : nullptr;
     hip::AttentionBatch batch{Q, ldq / 2, table, lengths, starts, table_width, tokens, group, scale * 1.4426950408889634f};
     hip::PagedCache cache{const_cast<uint8_t *>(k_cache), const_cast<uint8_t *>(v_cache), const_cast<float *>(k_scales), const_cast<float *>(v_scales),
@@ -541,8 +553,7 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     if (rc != 0 || plan.splits == 1) {
         return rc;
     }
-    const bool wave_a_row = plan.splits <= 16;
-    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, wave_a_row ? (rows + 3) / 4 : rows};
+    hip::JoinRows join{O, ldo / 2, partial, stats, starts, plan.splits, requests, q_heads, rows, join_blocks};
     const int joined = evaluate(p, wave_a_row ? kJoinWave : kJoinWorkgroup, who, stream, {{"batch", &batch}, {"rows", &join}});
     p->last_variant = plan.variant;
     return joined;
@@ -649,6 +660,9 @@ int gern_matvec4_run(gern_pipeline p, const void *X, int64_t ldx, const uint8_t 
     }
     const size_t variant = matvecVariant(M, N);
     const int64_t tile = 16 * kMatvecShapes[variant].column_tiles;
+    if (tooWide((N + tile - 1) / tile, 64 * kMatvecWaves)) {
+        return fail("gern_matvec4_run: N must be less than 2^27");
+    }
     hip::Activations x{X, ldx / 2, M};
     hip::Weights4 weights{codes, scales, zeros, N, K};
     hip::MatvecOut y{Y, ldy, (N + tile - 1) / tile};

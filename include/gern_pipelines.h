@@ -255,7 +255,9 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  * Keys on a page that is not in the cache (a table entry outside [0, pages), or
  * lengths[r] beyond the table) are left out, and gern_pipeline_faults is not 0
  * then.  What stands behind the last key, in its page or in the table, is not
- * used, whatever it is. */
+ * used, whatever it is; a key that is NaN makes the queries that see it NaN, a
+ * value that is NaN their result in its dimension.  Scales are finite, and scale
+ * * q . k within +-2^99. */
 #define GERN_CACHE_MAX_LENGTH (1 << 30)
 int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out);
 int gern_cache_attention_workspace(gern_pipeline p, int64_t tokens, int64_t requests, int64_t q_heads,

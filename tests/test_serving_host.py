@@ -209,3 +209,12 @@ def test_oracle_attention_is_softmax():
     o, tol = so.attention(q, k, v, np.ones(10), [0, 4, 10], 0.5)
     p = torch.softmax(torch.from_numpy(k @ q[2]) * 0.5, dim=0).numpy()
     assert np.all(o[0] == 0) and np.allclose(o[2], p @ v, rtol=1e-12) and np.all(tol[2] < 1e-2)
+
+
+def test_refuses_launches_of_too_many_threads(pipe):
+    """2^32 threads and more are no launch; such sizes are refused by name."""
+    lib = gern_amd.pipelines_lib()
+    refused(lib.gern_cache_write_run(*write_args(pipe, tokens=2 ** 25, heads=128, ldk=128 * 128, ldv=128 * 128)), "gern_cache_write_run", "2^23")
+    refused(lib.gern_matvec4_run(*matvec_args(pipe, M=1, N=2 ** 31 - 1, Y=1 << 50)), "gern_matvec4_run", "2^27")
+    refused(lib.gern_cache_attention_run(*attention_args(pipe, tokens=2 ** 25, requests=1, max_length=100000, O=1 << 52, workspace=1 << 40, workspace_bytes=2 ** 50)),
+            "gern_cache_attention_run", "2^24")
