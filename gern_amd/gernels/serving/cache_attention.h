@@ -424,28 +424,36 @@ struct AttentionRequest {
 };
 
 // NaN among the values of keys that some rows of a workgroup see and others do not is taken out (0 * NaN must not reach a
-// row that does not see the key) and put into the results of the rows that do when they are stored.  This does so for the
-// 16 keys at `base` and the rows [row, end).  It is rare, and reads the codes again: kept from the loop over the keys,
-// whatever would be noted there costs every call (64 requests: 162 to 177 us for 155).
+// row that does not see the key) and put into the results of the rows that do when all are stored.  This does so for the rows
+// [row, end) and the `count` keys at begin + offset, + step ... of their split: with `all` for all of them, which does no harm,
+// or for those that the first row does not see.  It is rare, and reads the codes again: noted in the loop over the keys, or
+// done right behind it, it would cost every call of few rows (64 requests: 177 and 160 us for 155).
 template<int D, int PAGE, class T>
-__device__ __forceinline__ void return_nan(AttentionRequest<D, PAGE, T> request, const AttentionPiece &piece, const KeyWalk<D, PAGE> &walk, int base,
-                                           int row, int end) {
-    // what this computes is not to be held in registers from before the loop over the keys
-    asm volatile("" : "+s"(request.group), "+s"(request.first), "+s"(request.splits));
-    const int lane = lane_id() + opaque_zero(), key = lane / 4, quarter = lane % 4;
-    const int id = walk.look_up(base);
-    if (id < 0 || id >= walk.cache.pages || base >= walk.length) {
-        return;
-    }
-    const uint32_t *v = walk.cache.v + ((int64_t)id * walk.cache.heads + walk.head) * (PAGE * D / 4);
-    const unsigned char *codes = reinterpret_cast<const unsigned char *>(v) + (base % PAGE + key) * D;
+__device__ __forceinline__ void return_nan(const AttentionRequest<D, PAGE, T> &request, const AttentionPiece &piece, const KeyWalk<D, PAGE> &walk, int row,
+                                           int end, int offset, int count, int step, bool all) {
+    const int most = row < end ? request.limit(end - 1) : 0, least = all ? 0 : request.limit(row);
+    const int64_t begin = (int64_t)request.split * piece.to.chunk;
+    const int last = request.split + 1 < request.splits ? (int)min(begin + piece.to.chunk, (int64_t)most) : most;
+    const int lane = lane_id() + opaque_zero(), quarter = lane % 4;
 #pragma unroll 1
-    for (int d = quarter * (D / 4); d < (quarter + 1) * (D / 4); d++) {
-        if ((codes[d] & 127) == 127) {
+    for (int at = (int)min(begin, (int64_t)most) + offset; at < last; at += step) {
 #pragma unroll 1
-            for (int r = row; r < end; r++) {
-                if (base + key < request.limit(r)) {
-                    request.put_nan(r, d, piece);
+        for (int key = at + lane / 4; key < at + count && at + count > least; key += 16) {
+            const int id = walk.pages[min(key / PAGE, walk.width - 1)];
+            if (id < 0 || id >= walk.cache.pages || key >= most) {
+                continue;
+            }
+            const uint32_t *v = walk.cache.v + ((int64_t)id * walk.cache.heads + walk.head) * (PAGE * D / 4);
+            const unsigned char *codes = reinterpret_cast<const unsigned char *>(v) + key % PAGE * D;
+#pragma unroll 1
+            for (int d = quarter * (D / 4); d < (quarter + 1) * (D / 4); d++) {
+                if ((codes[d] & 127) == 127) {
+#pragma unroll 1
+                    for (int r = row; r < end; r++) {
+                        if (key < request.limit(r)) {
+                            request.put_nan(r, d, piece);
+                        }
+                    }
                 }
             }
         }
@@ -490,6 +498,8 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
     const detail::KeyWalk<D, PAGE> walk = {cache, batch.table + piece.request * batch.width, piece.head, (int)batch.width, request.length, detail::opaque_zero()};
     const int tiles = (int)to.pieces / request.splits;
 
+    bool nan = false, any_missing = false;
+
     for (int tile = (int)piece.x / request.splits; tile * 16 < request.rows; tile += tiles) {
         const int row0 = tile * 16;
         detail::RowState<D, 1, T::kBf16> state;
@@ -501,11 +511,10 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         // `end` cuts a tile only where no row sees further: splits are whole tiles
         const int end = request.split + 1 < request.splits ? (int)min(begin + to.chunk, (int64_t)most) : most;
         constexpr int kStep = 32 * WAVES;
-        bool missing = false, nan = false;
+        bool missing = false;
         // Keys of the next step are loaded when this step's have been multiplied, values likewise, page numbers a step
         // before: no register is held for a load that waits, and none of the loads is waited for where it is issued.
-        const int first = (int)min(begin, (int64_t)most) + 32 * wave;
-        int base = first;
+        int base = (int)min(begin, (int64_t)most) + 32 * wave;
         detail::RawKeys<D> keys[2];
         int id[2] = {walk.look_up(base), walk.look_up(base + 16)};
         if (base < end) {
@@ -551,6 +560,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         if (missing && lane == 0) {
             atomicAdd(cache.faults, 1u);
         }
+        any_missing = any_missing || missing;
         state.l[0] = detail::sum_over_lane_groups(state.l[0]);
 
         // The wavefronts' parts meet in LDS; thread t then takes D / 16 values of row t / 16.
@@ -558,7 +568,6 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         constexpr int kPart = D / 16;
         __shared__ __attribute__((aligned(16))) float parts[WAVES][16][kPitch];
         __shared__ float part_m[WAVES][16], part_l[WAVES][16];
-        __shared__ int part_nan[WAVES];
         static_assert(WAVES >= 4, "256 threads share 16 rows");
         __syncthreads();  // the previous rows have been read
 #pragma unroll
@@ -572,7 +581,6 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         if (g == 0) {
             part_m[wave][c] = state.m[0];
             part_l[wave][c] = state.l[0];
-            part_nan[wave] = nan;
         }
         __syncthreads();
         const int at = threadIdx.x / 16, d = (threadIdx.x % 16) * kPart, row = row0 + at;
@@ -612,19 +620,11 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
                 }
             }
         }
-        int any_nan = part_nan[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            any_nan |= part_nan[w];
-        }
-        if (__builtin_amdgcn_readfirstlane(any_nan) != 0) {
-            __syncthreads();  // the results are stored
-            for (int at = first; nan && at < end; at += kStep) {
-                // (a tile was not whole either where its neighbour's page is missing)
-                for (int t = 0; t < 2 && (missing || at + 32 > least); t++) {
-                    detail::return_nan(request, piece, walk, at + 16 * t, row0, min(request.rows, row0 + 16));
-                }
-            }
+    }
+    __syncthreads();  // the results are stored
+    if (nan) {
+        for (int tile = (int)piece.x / request.splits; tile * 16 < request.rows; tile += tiles) {
+            detail::return_nan(request, piece, walk, tile * 16, min(request.rows, tile * 16 + 16), 32 * wave, 32, 32 * WAVES, any_missing);
         }
     }
 }
@@ -637,7 +637,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
 // is multiplied.  Bound by the vector ALU: per 16 rows and 32 keys a softmax of 8
 // scores a lane (8 exponentials at a quarter of the rate) stands against D / 8 matrix
 // instructions.  6 requests of 113 to 447 queries and 4032 to 5915 keys, 16 heads of
-// 64 on 4: 30.6 GFLOP in 97 us, 15 of them the join of six splits (213 us with keys
+// 64 on 4: 30.6 GFLOP in 101 us, 15 of them the join of six splits (213 us with keys
 // from memory for every wavefront).
 template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, class T>
 __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {
@@ -781,11 +781,7 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
         }
         if (nan) {
             __threadfence_block();  // this wavefront's results are stored
-            for (int at = begin; at < min(most, end); at += 16) {
-                if (at + 16 > least_of_all) {
-                    detail::return_nan(request, piece, walk, at, row0, min(request.rows, row0 + kRows));
-                }
-            }
+            detail::return_nan(request, piece, walk, row0, min(request.rows, row0 + kRows), 0, 16, 16, true);
         }
     }
 }
