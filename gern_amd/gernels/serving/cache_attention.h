@@ -9,10 +9,10 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax, in
 // fp32.  The value scale goes into the exponent: with
-//   y_j = z_j + log2 vs(j) (base 2) and m = max y,
-//   w_j = 2^(y_j - m) = p_j vs(j) / max(...) <= 1,
+//   y_j = z_j + log2 vs(j) (base 2) and m = max y - 15,
+//   w_j = 2^(y_j - m) = 2^15 p_j vs(j) / max(...) <= 2^15,
 // o = sum w_j vc_j / sum (w_j / vs(j)): the weights of the second product are at
-// most 1 whatever the scales are, and no product is scaled twice.
+// most 2^15 whatever the scales are, and no product is scaled twice.
 //
 // On the matrix cores, transposed so that nothing crosses lanes:
 //   S^T = K Q^T: 16 keys x 16 query rows a v_mfma_16x16x32; lane (g, c), c = lane
@@ -29,9 +29,13 @@
 // i holds dimension c D/16 + i and a lane ends up with D/4 consecutive values.
 //
 // Precision: codes go to bf16 / fp16 exactly.  Q.K is exact products in the
-// queries' type, summed in fp32.  The weights are rounded to fp16 (half a step is
-// 2^-11 of a weight) because fp16 holds every e4m3 code exactly, and their sum is
-// taken before rounding; bf16 weights would cost eight times that error.
+// queries' type, summed in fp32.  The weights are rounded to fp16 because fp16
+// holds every e4m3 code exactly, and their sum is taken before rounding; bf16
+// weights would cost eight times that error.  Half a step is 2^-11 of a weight down
+// to 2^-14, which is 2^-29 of the row's largest because that is 2^15; what is under
+// that is off by 2^-40 of the largest.  (With the largest at 1, 131072 keys that are
+// 13 under one whose page of values has 64 times their scale lost two thirds of what
+// they add up to.)  o <= 2^15 * 448 * 2^30 keys is far from the end of fp32.
 //
 // Bound by memory for few queries: 2 D bytes a key and head, read once (64 requests of
 // 4096 to 8192 keys, 8 heads of 128: 788 MB in 155 us, 5.1 TB/s; a copy of 1 GiB
@@ -65,7 +69,7 @@ struct AttentionOut {
     uint32_t *out;       // two values a word
     int64_t out_pitch;   // words
     float *partial;      // [splits, tokens * query heads, D], with splits > 1
-    float *stats;        // [splits, tokens * query heads, 2]: maximum, sum
+    float *stats;        // [splits, tokens * query heads, 2]: maximum less kWeightBits, sum
     int64_t splits;      // of the keys, `chunk` each (the last one takes the rest)
     int64_t chunk;
     int64_t pieces;      // workgroups per request and head: row tiles * splits
@@ -126,6 +130,9 @@ __device__ __forceinline__ int opaque_zero() {
 
 // Below every score; finite, so that a row that has seen nothing yet gives 2^(-inf - m) = 0.
 constexpr float kLowest = -1.0e30f;
+
+// log2 of a row's largest weight: the largest power of two of fp16.
+constexpr float kWeightBits = 15.0f;
 
 // 16 keys of one head of the cache, as they are in memory.
 template<int D>
@@ -241,7 +248,7 @@ template<int D, int R, bool BF16>
 struct RowState {
     Frag q[R][D / 32];     // lane (g, c): row c, dimensions g D/4 + 8 s ..
     f32x4 o[R][D / 16];    // lane (g, c): row c, o[.][i][e] is dimension (4 g + e) D/16 + i
-    float m[R], l[R];      // maximum over the row, sum over this lane's keys
+    float m[R], l[R];      // maximum over the row less kWeightBits, sum over this lane's keys
     int limit[R];          // keys that row c sees
 
     __device__ __forceinline__ void clear() {
@@ -306,7 +313,7 @@ struct RowState {
                 const float score = __builtin_fmaf(most, scales[t].k, scales[t].up);
                 top = t == 0 ? score : larger(top, score);
             }
-            top = max_over_lane_groups(top);
+            top = max_over_lane_groups(top) - kWeightBits;
             if (__ballot(top > m[r]) != 0) {
                 const float now = larger(top, m[r]);
                 const float shrink = __builtin_amdgcn_exp2f(m[r] - now);

@@ -247,8 +247,10 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  * stride ldo; rows of Q in no request are left alone in O.  O may be Q (with the
  * same stride); it shares memory with nothing else that the call reads.
  * max_queries and max_length tell the most queries and keys of one request; the
- * division of the work and the workspace depend on them and the results do not
- * (more are computed, too, only slower).  The workspace
+ * division of the work and the workspace depend on them, results only in their
+ * rounding (more are computed, too, only slower).  A weight (a value's share
+ * times its scale) is rounded to 11 bits; what is under 2^-29 of a row's largest
+ * keeps fewer, and what is under 2^-40 counts as 0.  The workspace
  * (gern_cache_attention_workspace bytes, 16-byte aligned, any content) is the
  * call's from its launch to its end: calls that overlap in time need one each.
  * One launch, or two where the keys are split among workgroups.

@@ -1,0 +1,99 @@
+"""The operators of a serving step where weights, scales and activations leave the ordinary range, against 64 bits."""
+import numpy as np
+import pytest
+
+from test_gpu_serving import E4M3, HALF_STEP, gpu, i32, torch  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def code_of(x):
+    """The e4m3 code nearest to each value."""
+    import torch
+    return torch.from_numpy(np.asarray(x, dtype=np.float32)).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+
+
+def attention_of(q, k, v, v_scales, limits, scale):
+    """One head of one request, as serving_oracle.attention: the result, and how far a kernel may be from it before it rounds
+    its result.  Weights are p * (scale of the value), the largest of a row 2^15: fp16 keeps 11 bits of them down to 2^-14, that
+    is 2^-29 of the largest, and is off by 2^-25, that is 2^-40 of the largest, under it."""
+    n, dim = q.shape
+    o, tol = np.zeros((n, dim)), np.zeros((n, dim))
+    codes = np.abs(v) / np.where(v_scales > 0, v_scales, 1.0)[:, None]
+    for i in range(n):
+        m = int(limits[i])
+        if m <= 0:
+            continue
+        z = (k[:m] @ q[i]) * scale
+        exponent = ((dim / 32 + 8) * 2.0 ** -24 * (np.abs(k[:m]) @ np.abs(q[i])) * scale + 8 * 2.0 ** -24 * (np.abs(z) + 128)).max()
+        p = np.exp(z - z.max())
+        p /= p.sum()
+        o[i] = p @ v[:m]
+        tol[i] = (2.0 ** -11 + 2 * exponent + (m / 32 + 16) * 2.0 ** -24) * (p @ np.abs(v[:m])) + 2.0 ** -40 * codes[:m].sum(axis=0) * (p * v_scales[:m]).max()
+    return o, tol
+
+
+class Request:
+    """One request over pages in order, one head of keys; kc and vc [length, dim] codes, scales a page."""
+
+    def __init__(self, torch, dtype, page, kc, vc, k_scales, v_scales, q):
+        length, dim = kc.shape
+        pages = -(-length // page)
+        t = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+        self.page, self.dim, self.length, self.dtype = page, dim, length, dtype
+        codes = np.zeros((2, pages, 1, page, dim), dtype=np.uint8)
+        codes.reshape(2, -1, dim)[:, :length] = np.stack([kc, vc])
+        self.k_cache, self.v_cache = (torch.from_numpy(c).cuda() for c in codes)
+        scales = np.stack([k_scales, v_scales]).astype(np.float32)
+        self.k_scales, self.v_scales = (torch.from_numpy(s[:, None].copy()).cuda() for s in scales)
+        self.q = torch.from_numpy(q).to(t)  # [queries, heads, dim]
+        of = np.repeat(scales.astype(np.float64), page, axis=1)[:, :length]
+        self.k, self.v, self.vs = E4M3[kc] * of[0][:, None], E4M3[vc] * of[1][:, None], of[1]
+
+    def run(self, torch, gpu, scale, few=True, splits=True):
+        """The result.  `few`: the program for few rows.  Not `splits`: as among 1024 workgroups, whose keys are not divided (requests
+        without tokens, or room for more queries)."""
+        queries, heads, dim = self.q.shape
+        requests = 1 if splits or not few else 1024
+        max_queries = queries if few else 100 if splits else 1 << 17
+        a = gpu("CacheAttention", head_dim=dim, page_size=self.page, dtype=self.dtype)
+        n = a.workspace_bytes(queries, requests, heads, 1, max_queries, self.length)
+        assert (n > 0) == splits
+        table = np.tile(np.arange(self.k_cache.shape[0]), (requests, 1))
+        out = torch.zeros((queries, heads, dim), dtype=self.q.dtype, device="cuda")
+        a(self.q.cuda(), self.k_cache, self.v_cache, self.k_scales, self.v_scales, i32(torch, table), i32(torch, [self.length] + [0] * (requests - 1)),
+          i32(torch, [0] + [queries] * requests), out, scale, max_queries=max_queries, max_length=self.length,
+          workspace=torch.empty(n, dtype=torch.uint8, device="cuda"))
+        torch.cuda.synchronize()
+        assert a.faults() == 0
+        return out.double().cpu().numpy()
+
+    def check(self, out, scale):
+        queries, heads, _ = self.q.shape
+        for h in range(heads):
+            want, tol = attention_of(self.q[:, h].double().numpy(), self.k, self.v, self.vs, self.length - queries + np.arange(queries) + 1, scale)
+            tol = tol + HALF_STEP[self.dtype] * (np.abs(want) + tol) + (2.0 ** -25 if self.dtype == "f16" else 2.0 ** -134)
+            assert np.all(np.abs(out[:, h] - want) <= tol), float((np.abs(out[:, h] - want) / tol).max())
+
+
+@pytest.mark.parametrize("few, splits", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("length, above, ratio, spread", [(32768, 12, 16, 0.0), (131072, 13, 64, 0.0), (131072, 13, 64, 1.0), (20000, 9, 2 ** 12, 0.5)])
+def test_attention_keeps_small_weights(torch, gpu, few, splits, length, above, ratio, spread):  # noqa: F811
+    """One key far above the others, whose value is 0 in most dimensions, on a page of a larger scale: what the others add up
+    to there is the result."""
+    dim, page, queries = 64, 16, 2 if few else 100
+    rs = np.random.RandomState(length + above)
+    q = rs.normal(size=(queries, 2, dim))
+    q[..., 0] = 1.0
+    k = rs.normal(size=(length, dim)) * spread / dim ** 0.5
+    k[:, 0], k[0] = 0.0, 0.0
+    k[0, 0] = above
+    pages = -(-length // page)
+    v_scales = np.full(pages, 2.0 ** -4)
+    v_scales[0] *= ratio
+    v = 32.0 * (1.0 + 0.3 * rs.normal(size=(length, dim)))  # in units of their page's scale
+    v[:page] /= ratio
+    v[0] = 0.0
+    v[0, 0] = 256.0
+    r = Request(torch, "bf16", page, code_of(k), code_of(v), np.ones(pages), v_scales, q)
+    r.check(r.run(torch, gpu, 1.0, few, splits), 1.0)
