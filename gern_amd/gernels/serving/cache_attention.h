@@ -868,9 +868,8 @@ __device__ __forceinline__ void join_splits(const AttentionBatchOf<T> &, const J
     auto add = [&](int s, float w) {
 #pragma unroll
         for (int i = 0; i < kPart; i++) {
-            // a split without any of the row's keys wrote no part
-            const float p = part[s * to.rows * D + i];
-            x[i] = __builtin_fmaf(w != 0.0f ? p : 0.0f, w, x[i]);
+            // a weight of 0 as well: every split wrote its part, zeros where it saw nothing, and NaN is to stay
+            x[i] = __builtin_fmaf(part[s * to.rows * D + i], w, x[i]);
         }
     };
     if constexpr (PER_ROW == 1) {

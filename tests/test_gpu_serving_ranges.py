@@ -97,3 +97,26 @@ def test_attention_keeps_small_weights(torch, gpu, few, splits, length, above, r
     v[0, 0] = 256.0
     r = Request(torch, "bf16", page, code_of(k), code_of(v), np.ones(pages), v_scales, q)
     r.check(r.run(torch, gpu, 1.0, few, splits), 1.0)
+
+
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("length", [8000, 9000])
+def test_attention_nan_in_keys_of_no_weight(torch, gpu, few, length):  # noqa: F811
+    """A value that is NaN makes its dimension of the result NaN also where its part of the keys has a weight of 0 beside the
+    others (16 parts, joined by a wavefront, and 18, by a workgroup)."""
+    dim, page, queries, high = 64, 32, 2 if few else 100, length - 700
+    rs = np.random.RandomState(length)
+    q = rs.normal(size=(queries, 2, dim))
+    q[..., 0] = 1.0
+    k = np.zeros((length, dim))
+    k[high, 0] = 144.0  # 207 in base 2: 2^-207 of it is 0
+    v = code_of(rs.normal(size=(length, dim)))
+    v[100, 5], v[101, 63] = 127, 255
+    pages = -(-length // page)
+    for nan in (True, False):
+        out = Request(torch, "bf16", page, code_of(k), v, np.ones(pages), np.ones(pages), q).run(torch, gpu, 1.0, few)
+        odd = np.zeros(dim, dtype=bool)
+        odd[[5, 63]] = nan
+        assert np.array_equal(np.isnan(out), np.broadcast_to(odd, out.shape))
+        assert np.array_equal(out[..., ~odd], np.broadcast_to(E4M3[v[high]][~odd], out[..., ~odd].shape))
+        v[100, 5], v[101, 63] = 0, 0
