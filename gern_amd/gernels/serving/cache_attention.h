@@ -134,6 +134,10 @@ constexpr float kLowest = -1.0e30f;
 // log2 of a row's largest weight: the largest power of two of fp16.
 constexpr float kWeightBits = 15.0f;
 
+// The least scale of values, 2^-80: 2^30 weights of 2^15, each over it, add up to less than 2^126.  What is under it
+// counts as 0: the softmax takes it as this, and the values are 0.
+constexpr float kLeastValueScale = 8.271806125530277e-25f;
+
 // 16 keys of one head of the cache, as they are in memory.
 template<int D>
 struct RawKeys {
@@ -170,6 +174,20 @@ struct RawKeys {
             }
         }
     }
+    // Whether the values' scale counts as 0.
+    __device__ __forceinline__ bool without_scale() const {
+        return as_float(__builtin_amdgcn_readfirstlane(as_int(v_scale))) < kLeastValueScale;
+    }
+    __device__ __forceinline__ void clear_values_without_scale() {
+        const uint32_t keep = without_scale() ? 0u : 0xffffffffu;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int w = 0; w < D / 64; w++) {
+                v[j][w] &= keep;
+            }
+        }
+    }
     // Makes 0 of the values that are NaN (codes 127 and 255); whether there were any.
     __device__ __forceinline__ bool take_nan() {
         uint32_t found = 0;
@@ -195,10 +213,9 @@ struct TileScales {
 };
 template<int D>
 __device__ __forceinline__ TileScales scales_of(const RawKeys<D> &tile, float scale) {
-    // A scale of values under 2^-64 counts as that: its codes are zero, or too small to matter.  The scale of the
-    // scores stays above zero because -infinity, a key that is not seen, is multiplied by it.
+    // The scale of the scores stays above zero because -infinity, a key that is not seen, is multiplied by it.
     const float k = tile.k_scale * scale, v = tile.v_scale;
-    const float vs = !tile.there ? 1.0f : v < 5.421010862e-20f ? 5.421010862e-20f : v;
+    const float vs = !tile.there ? 1.0f : v < kLeastValueScale ? kLeastValueScale : v;
     return {!tile.there ? 1.0f : k < 1.0e-30f ? 1.0e-30f : k, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
 }
 
@@ -505,7 +522,7 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
     const detail::KeyWalk<D, PAGE> walk = {cache, batch.table + piece.request * batch.width, piece.head, (int)batch.width, request.length, detail::opaque_zero()};
     const int tiles = (int)to.pieces / request.splits;
 
-    bool nan = false, any_missing = false;
+    int notes = 0;  // 1: NaN was taken, 2: keys that all rows see were not taken whole
 
     for (int tile = (int)piece.x / request.splits; tile * 16 < request.rows; tile += tiles) {
         const int row0 = tile * 16;
@@ -534,8 +551,9 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         }
         while (base < end) {
             const bool there[2] = {keys[0].there, keys[1].there};
-            const bool whole = base + 32 <= least && there[0] && there[1];
+            const bool all_see = base + 32 <= least, whole = all_see && there[0] && there[1] && !keys[0].without_scale() && !keys[1].without_scale();
             missing = missing || !there[0] || (!there[1] && base + 16 < end);
+            notes |= all_see && !whole ? 2 : 0;
             const bool more = base + kStep < end;
             state.template add<1>(
                 base, whole, [&](int t, int i) { return keys[t].template key_frag<T::kBf16>(i); },
@@ -544,8 +562,10 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
                     if (!whole) {
                         keys[0].clear_values_behind(base, request.length);
                         keys[1].clear_values_behind(base + 16, request.length);
-                        nan = keys[0].take_nan() || nan;
-                        nan = keys[1].take_nan() || nan;
+                        notes |= keys[0].take_nan() ? 1 : 0;
+                        notes |= keys[1].take_nan() ? 1 : 0;
+                        keys[0].clear_values_without_scale();
+                        keys[1].clear_values_without_scale();
                     }
                     if (more) {
                         walk.load_keys(keys[0], base + kStep, id[0]);
@@ -567,7 +587,6 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         if (missing && lane == 0) {
             atomicAdd(cache.faults, 1u);
         }
-        any_missing = any_missing || missing;
         state.l[0] = detail::sum_over_lane_groups(state.l[0]);
 
         // The wavefronts' parts meet in LDS; thread t then takes D / 16 values of row t / 16.
@@ -629,9 +648,9 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
         }
     }
     __syncthreads();  // the results are stored
-    if (nan) {
+    if ((notes & 1) != 0) {
         for (int tile = (int)piece.x / request.splits; tile * 16 < request.rows; tile += tiles) {
-            detail::return_nan(request, piece, walk, tile * 16, min(request.rows, tile * 16 + 16), 32 * wave, 32, 32 * WAVES, any_missing);
+            detail::return_nan(request, piece, walk, tile * 16, min(request.rows, tile * 16 + 16), 32 * wave, 32, 32 * WAVES, (notes & 2) != 0);
         }
     }
 }
@@ -680,9 +699,10 @@ __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batc
         detail::RawKeys<D> keys;
         auto stage = [&](int buffer, int base) {
             bool taken = false;
-            if (!keys.there || base + 16 > least_of_all) {
+            if (!keys.there || keys.without_scale() || base + 16 > least_of_all) {
                 keys.clear_values_behind(base, request.length);
                 taken = keys.take_nan();
+                keys.clear_values_without_scale();
             }
 #pragma unroll
             for (int i = 0; i < D / 32; i++) {

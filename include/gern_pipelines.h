@@ -259,7 +259,10 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  * then.  What stands behind the last key, in its page or in the table, is not
  * used, whatever it is; a key that is NaN makes the queries that see it NaN, a
  * value that is NaN their result in its dimension.  Scales are finite, and scale
- * * q . k within +-2^99. */
+ * * q . k within +-2^99.  Scales of values are at most 2^120; those under 2^-80
+ * count as 0 (their keys weigh in the softmax and their values are 0), and the
+ * others of a request are within 2^100 of one another and of 2^-80 where it has
+ * such pages. */
 #define GERN_CACHE_MAX_LENGTH (1 << 30)
 int gern_cache_attention_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out);
 int gern_cache_attention_workspace(gern_pipeline p, int64_t tokens, int64_t requests, int64_t q_heads,

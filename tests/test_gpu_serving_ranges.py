@@ -120,3 +120,42 @@ def test_attention_nan_in_keys_of_no_weight(torch, gpu, few, length):  # noqa: F
         assert np.array_equal(np.isnan(out), np.broadcast_to(odd, out.shape))
         assert np.array_equal(out[..., ~odd], np.broadcast_to(E4M3[v[high]][~odd], out[..., ~odd].shape))
         v[100, 5], v[101, 63] = 0, 0
+
+
+def random_request(torch, dtype, dim, page, length, v_scales, queries, heads=2, seed=0):  # noqa: F811
+    rs = np.random.RandomState(seed)
+    k, v = (code_of(rs.normal(size=(length, dim)) * 16) for _ in range(2))
+    return Request(torch, dtype, page, k, v, np.full(-(-length // page), 1 / 64), v_scales, rs.normal(size=(queries, heads, dim)))
+
+
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("dim, length, splits", [(64, 600, False), (128, 5000, True), (192, 200, False), (256, 3000, True)])
+def test_attention_small_scales_of_values(torch, gpu, few, dim, length, splits):  # noqa: F811
+    """Scales of values down to 2^-80; what is under that, 0 among it, weighs in the softmax and adds nothing."""
+    page, queries, scale = 16, 2 if few else 90, dim ** -0.5
+    pages = -(-length // page)
+    rs = np.random.RandomState(length)
+    for scales in (np.full(pages, 2.0 ** -70), np.full(pages, 1.37 * 2.0 ** -80), np.exp2(rs.randint(-80, -60, pages)), np.exp2(rs.randint(-80, 4, pages))):
+        r = random_request(torch, "bf16", dim, page, length, scales, queries, seed=length)
+        r.check(r.run(torch, gpu, scale, few, splits), scale)
+        none = rs.rand(pages) < 0.4
+        for small in (0.0, 2.0 ** -140, 2.0 ** -81):
+            r.v_scales[torch.from_numpy(none).cuda()] = small
+            r.v[np.repeat(none, page)[:length]] = 0.0
+            r.check(r.run(torch, gpu, scale, few, splits), scale)
+
+
+@pytest.mark.parametrize("few", [True, False])
+@pytest.mark.parametrize("dim, length, splits", [(64, 600, False), (128, 5000, True), (256, 100, False)])
+def test_attention_values_of_no_scale(torch, gpu, few, dim, length, splits):  # noqa: F811
+    """No page has a scale: the result is 0, but for dimensions in which a key that is seen has NaN."""
+    page, queries = 32, 3 if few else 90
+    r = random_request(torch, "bf16", dim, page, length, np.zeros(-(-length // page)), queries, seed=length)
+    assert np.all(r.run(torch, gpu, 0.1, few, splits) == 0.0)
+    codes = r.v_cache.view(-1, dim)
+    codes[7, 3], codes[length - 2, dim - 1] = 127, 255  # the last but one key: all but the first `queries - 2` see it
+    out = r.run(torch, gpu, 0.1, few, splits)
+    odd = np.zeros(out.shape, dtype=bool)
+    odd[:, :, 3] = True
+    odd[queries - 2:, :, dim - 1] = True
+    assert np.array_equal(np.isnan(out), odd) and np.all(out[~odd] == 0.0)
