@@ -213,10 +213,11 @@ struct TileScales {
 };
 template<int D>
 __device__ __forceinline__ TileScales scales_of(const RawKeys<D> &tile, float scale) {
-    // The scale of the scores stays above zero because -infinity, a key that is not seen, is multiplied by it.
+    // The scale of the scores stays above zero because -infinity, a key that is not seen, is multiplied by it: at 2^-126 a
+    // score is 0 but for products of queries and codes beyond 2^100.
     const float k = tile.k_scale * scale, v = tile.v_scale;
     const float vs = !tile.there ? 1.0f : v < kLeastValueScale ? kLeastValueScale : v;
-    return {!tile.there ? 1.0f : k < 1.0e-30f ? 1.0e-30f : k, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
+    return {!tile.there ? 1.0f : k < 1.17549435e-38f ? 1.17549435e-38f : k, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
 }
 
 // What a wavefront needs to walk the keys of one request and head.

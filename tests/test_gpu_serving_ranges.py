@@ -159,3 +159,17 @@ def test_attention_values_of_no_scale(torch, gpu, few, dim, length, splits):  # 
     odd[:, :, 3] = True
     odd[queries - 2:, :, dim - 1] = True
     assert np.array_equal(np.isnan(out), odd) and np.all(out[~odd] == 0.0)
+
+
+@pytest.mark.parametrize("few", [True, False])
+def test_attention_small_scales_of_keys(torch, gpu, few):  # noqa: F811
+    """Large queries and keys of a small scale: the scores are ordinary.  Keys of scale 0 have the score 0."""
+    dim, page, length, queries = 128, 16, 400, 2 if few else 90
+    rs = np.random.RandomState(3)
+    k, v = (code_of(rs.normal(size=(length, dim)) * 16) for _ in range(2))
+    q = rs.normal(size=(queries, 2, dim)) * 2.0 ** 100
+    pages = -(-length // page)
+    k_scales = np.exp2(rs.randint(-108, -103, pages))
+    k_scales[3] = 0.0
+    r = Request(torch, "bf16", page, k, v, k_scales, np.ones(pages), q)
+    r.check(r.run(torch, gpu, dim ** -0.5, few, False), dim ** -0.5)
