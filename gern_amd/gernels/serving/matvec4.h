@@ -12,11 +12,13 @@
 // then a whole number of steps, and its scale multiplies fp32 sums, not weights.
 //
 // A code becomes a 16-bit float without arithmetic: or'ed into the mantissa of
-// 128 (bf16, lowest bits) or 64 (fp16, bits 4 - 7) it stands for 128 + q or 64 + q
-// exactly, two codes (nibbles i and i + 4) an instruction.  x is laid out in pairs
+// a power of two (bf16: 2^-9, lowest bits, fp16: 64, bits 4 - 7) it stands for
+// 2^-16 (128 + q) or 64 + q exactly, two codes (nibbles i and i + 4) an
+// instruction.  The 2^-16, taken back at the end, keeps a group's sums of bf16
+// activations finite whatever these are (128 of them times 128 + 255 at most).  x is laid out in pairs
 // (i, i + 4) to match, and the offset leaves with the zero point:
 // sum x (128 + q) - (128 + z) sum x.  The sum of x comes from one more matrix
-// instruction, against ones, for all columns.  The offset costs fp32 rounding of a
+// instruction, against ones (2^-9 again), for all columns.  The offset costs fp32 rounding of a
 // sum 128 / 4.6 (the spread of q - z) times larger: 2^-24 * 28, 2^-19.2 of the
 // result's size against the 2^-8 (bf16) or 2^-11 (fp16) of its last rounding.
 //
@@ -85,15 +87,18 @@ __device__ __forceinline__ void transpose_lane_groups(uint32_t w[4]) {
     }
 }
 
-// offset + code for the eight codes of a word, in pairs (i, i + 4).
+// unit * (offset + code) for the eight codes of a word, in pairs (i, i + 4); `one` stands for one in the sum of x, and is a
+// power of two (bits `ones`, twice).
 template<bool BF16>
 struct CodeOffset {
     static constexpr float value = BF16 ? 128.0f : 64.0f;
+    static constexpr float unit = BF16 ? 0x1p-16f : 1.0f, one = BF16 ? 0x1p-9f : 1.0f;
+    static constexpr uint32_t ones = BF16 ? 0x3b003b00u : 0x3c003c00u;
 };
 // `offsets` is code_offsets<BF16>(): in a register, so that `and` and `or` are one instruction (two literals do not fit).
 template<bool BF16>
 __device__ __forceinline__ uint32_t code_offsets() {
-    uint32_t two = BF16 ? 0x43004300u : 0x54005400u;
+    uint32_t two = BF16 ? 0x3b003b00u : 0x54005400u;
     asm volatile("" : "+v"(two));
     return two;
 }
@@ -215,7 +220,8 @@ __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const W
             }
         }
     }
-    constexpr uint32_t kOnes = kBf16 ? 0x3f803f80u : 0x3c003c00u;
+    using Offset = detail::CodeOffset<kBf16>;
+    constexpr uint32_t kOnes = Offset::ones;
     const detail::Frag ones = {{kOnes, kOnes, kOnes, kOnes}};
     const detail::f32x4 nothing = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t offsets = detail::code_offsets<kBf16>();
@@ -322,7 +328,8 @@ __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const W
                     }
                 }
                 const float scale = half_to_float<T>(scale_zero[t] & 0xffffu);
-                const float zero = -((with_zeros ? (float)(scale_zero[t] >> 16) : 8.0f) + detail::CodeOffset<kBf16>::value);
+                constexpr float kPerOne = Offset::unit / Offset::one;
+                const float zero = __builtin_fmaf(with_zeros ? (float)(scale_zero[t] >> 16) : 8.0f, -kPerOne, -kPerOne * Offset::value);
 #pragma unroll
                 for (int r = 0; r < kRowTiles; r++) {
 #pragma unroll
@@ -388,6 +395,7 @@ __device__ __forceinline__ void multiply_4bit(const ActivationsOf<T> &a, const W
         for (int w = 0; w < WAVES; w++) {
             y += parts[w][i / kWaveSize][i % kWaveSize];
         }
+        y *= 1.0f / Offset::unit;
         const int from = i % kWaveSize, tile = i / kWaveSize / kSums, e = i / kWaveSize % kSums;
         const int64_t m = kFew ? from / 16 : 16 * (tile % kRowTiles) + 4 * (from / 16) + e, n = n0 + 16 * (tile / kRowTiles) + from % 16;
         if (m < a.rows && n < weights.n) {

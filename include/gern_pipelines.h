@@ -281,8 +281,10 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
  * the lower half of a byte is the even column, 16-byte aligned; scales:
  * [K / group, N] in `type`; zeros: [K / group, N] bytes of 0 .. 255, or NULL: 8
  * everywhere; Y: [M, N] in `type`, row stride ldy.  group is 32, 64 or 128 and
- * divides K, which is at most GERN_MATVEC4_MAX_COLUMNS.  Sums are fp32, rounded once.  A row of X with an infinity gives
- * NaN.  For more rows the products, and no longer the weights, are the work:
+ * divides K, which is at most GERN_MATVEC4_MAX_COLUMNS.  Sums
+ * are fp32, rounded once; those of bf16 are taken of 2^-16 of the products, so
+ * that no finite X overflows on the way, and X under 2^-116 keeps fewer bits.
+ * A row of X with an infinity gives NaN.  For more rows the products, and no longer the weights, are the work:
  * that is gern_gemm_run's. */
 #define GERN_MATVEC4_MAX_ROWS 64
 #define GERN_MATVEC4_MAX_COLUMNS (1 << 24)

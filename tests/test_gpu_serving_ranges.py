@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+import serving_oracle as so
 from test_gpu_serving import E4M3, HALF_STEP, gpu, i32, torch  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -173,3 +174,43 @@ def test_attention_small_scales_of_keys(torch, gpu, few):  # noqa: F811
     k_scales[3] = 0.0
     r = Request(torch, "bf16", page, k, v, k_scales, np.ones(pages), q)
     r.check(r.run(torch, gpu, dim ** -0.5, few, False), dim ** -0.5)
+
+
+@pytest.mark.parametrize("m", [1, 3, 4, 5, 16, 20, 40])
+@pytest.mark.parametrize("group, k", [(32, 96), (64, 320), (128, 1024)])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_matvec_large_activations(torch, gpu, m, group, k, zeros):  # noqa: F811
+    """Activations up to the largest of bf16 whose products with the weights are finite: no sum on the way overflows."""
+    rs = np.random.RandomState(m + k)
+    n = 50
+    for x, size in ((rs.normal(size=(m, k)) * 1e36, 0.01), (np.full((m, k), 2.0 ** 127), 2.0 ** -20), (rs.choice([-3.3e38, 3.3e38], (m, k)), 2.0 ** -20)):
+        x = torch.from_numpy(x).bfloat16()
+        codes = rs.randint(0, 256, (n, k // 2)).astype(np.uint8)
+        scales = torch.from_numpy(rs.uniform(0.5, 2.0, (k // group, n)) * size).bfloat16()
+        z = rs.randint(0, 256, (k // group, n)).astype(np.uint8) if zeros else np.full((k // group, n), 8, dtype=np.uint8)
+        y = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+        gpu("Matvec4", group=group, dtype="bf16")(x.cuda(), torch.from_numpy(codes).cuda(), scales.cuda(), y, zeros=torch.from_numpy(z).cuda() if zeros else None)
+        torch.cuda.synchronize()
+        want, tol = so.matvec4(x.double().numpy(), codes, scales.double().numpy(), z.astype(np.float64), group, 128)
+        assert np.abs(want).max() < 3e38
+        assert np.all(np.abs(y.double().cpu().numpy() - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol))
+
+
+@pytest.mark.parametrize("m", [1, 4, 13, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_matvec_small_activations(torch, gpu, m, group):  # noqa: F811
+    """Activations around 2^-112: the sums are taken of 2^-16 of the products, in steps of 2^-149 at least."""
+    rs = np.random.RandomState(m + group)
+    n, k = 50, 1024
+    x = torch.from_numpy(rs.normal(size=(m, k)) * 2.0 ** -112).bfloat16()
+    codes = rs.randint(0, 256, (n, k // 2)).astype(np.uint8)
+    scales = torch.from_numpy(rs.uniform(0.5, 2.0, (k // group, n))).bfloat16()
+    z = rs.randint(0, 256, (k // group, n)).astype(np.uint8)
+    y = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+    gpu("Matvec4", group=group, dtype="bf16")(x.cuda(), torch.from_numpy(codes).cuda(), scales.cuda(), y, zeros=torch.from_numpy(z).cuda())
+    torch.cuda.synchronize()
+    want, tol = so.matvec4(x.double().numpy(), codes, scales.double().numpy(), z.astype(np.float64), group, 128)
+    # half steps of 2^-149: 8 + group / 32 of a group's products, as many of its sum of x, which counts 3 times (383 / 128), and one
+    # where the group is added; all times 2^16
+    steps = 2.0 ** -150 * (4 * (8 + group / 32) + 1) * scales.double().numpy().sum(axis=0) * 2.0 ** 16
+    assert np.all(np.abs(y.double().cpu().numpy() - want) <= tol + steps + HALF_STEP["bf16"] * (np.abs(want) + tol + steps))
