@@ -320,7 +320,10 @@ def _expect(ok, what):
 
 class _ServingPipeline(_Pipeline):
     """A pipeline of torch tensors: it checks types, layouts and devices before it hands addresses to the C ABI.  The
-    checks are written out for what they cost: a decoding step makes several of these calls of a few microseconds."""
+    checks are written out for what they cost: a decoding step makes several of these calls of a few microseconds.
+
+    A call runs on `stream`, a HIP stream's address (0: the default stream), by default on torch's current stream, in order
+    with the torch operations before and after it, also where torch captures a graph."""
 
     def __init__(self, dtype=None):
         super().__init__()
@@ -329,6 +332,8 @@ class _ServingPipeline(_Pipeline):
         self._int32_type, self._uint8, self._float32 = torch.int32, torch.uint8, torch.float32
         self._code_types = (torch.float8_e4m3fn, torch.uint8)
         self._half = {"bf16": torch.bfloat16, "f16": torch.float16, None: None}[dtype]
+        # the address of a device's current stream: torch.cuda.current_stream makes an object around it, for a microsecond
+        self._current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
     def _on_gpu(self, *tensors):
         """All on the GPU that the pipeline was created on (a kernel runs where its code was loaded)."""
@@ -391,7 +396,7 @@ class PageTable(_ServingPipeline):
         self._on_gpu(cached, added, free_pages, free_count, table, lengths, starts, slots, counts)
         _check(self._run(self.h, cached.data_ptr(), added.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
                          table.data_ptr(), table.shape[1], lengths.data_ptr(), starts.data_ptr(), slots.data_ptr(), slots.shape[0], counts.data_ptr(),
-                         stream))
+                         self._current_stream(self._device) if stream is None else stream))
         return table, slots
 
 
@@ -413,7 +418,7 @@ class CacheWrite(_ServingPipeline):
         _expect(slots.dim() == 1 and k.shape == v.shape == (slots.shape[0], heads, self.head_dim), "slots must be [tokens], k and v [tokens, heads, head_dim]")
         self._on_gpu(k, v, slots, k_cache, v_cache, k_scales, v_scales)
         _check(self._run(self.h, k.data_ptr(), ldk, v.data_ptr(), ldv, slots.data_ptr(), slots.shape[0], heads, k_cache.data_ptr(), v_cache.data_ptr(),
-                         k_scales.data_ptr(), v_scales.data_ptr(), pages, stream))
+                         k_scales.data_ptr(), v_scales.data_ptr(), pages, self._current_stream(self._device) if stream is None else stream))
 
 
 class CacheAttention(_ServingPipeline):
@@ -451,7 +456,8 @@ class CacheAttention(_ServingPipeline):
             at, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         _check(self._run(self.h, q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), pages, table.data_ptr(),
                          width[1], lengths.data_ptr(), starts.data_ptr(), width[0], shape[0], shape[1], heads, out.data_ptr(), ldo, scale, max_queries,
-                         width[1] * self.page_size if max_length is None else max_length, at, size, stream))
+                         width[1] * self.page_size if max_length is None else max_length, at, size,
+                         self._current_stream(self._device) if stream is None else stream))
         return out
 
 
@@ -479,5 +485,6 @@ class Matvec4(_ServingPipeline):
             self._on_gpu(zeros)
             at = zeros.data_ptr()
         self._on_gpu(x, codes, scales, y)
-        _check(self._run(self.h, x.data_ptr(), ldx, codes.data_ptr(), scales.data_ptr(), at, y.data_ptr(), ldy, m, n, k, stream))
+        _check(self._run(self.h, x.data_ptr(), ldx, codes.data_ptr(), scales.data_ptr(), at, y.data_ptr(), ldy, m, n, k,
+                         self._current_stream(self._device) if stream is None else stream))
         return y
