@@ -7,6 +7,7 @@
 
 #include "annot/matvec4.h"
 #include "annot/paged_cache.h"
+#include "csrc/memory_ranges.h"
 #include "gern_hip.h"
 
 #include <algorithm>
@@ -17,6 +18,8 @@ using namespace gern;
 using gern_detail::fail;
 using gern_detail::failHip;
 using gern_detail::finish;
+using gern_detail::overlap;
+using gern_detail::Rows;
 
 namespace {
 
@@ -80,6 +83,10 @@ bool usable(gern_pipeline p, gern_pipeline_s::Kind kind) {
     return p != nullptr && p->kind == kind;
 }
 
+bool compileOnly(gern_pipeline p) {
+    return p->variants[0].runner == nullptr;
+}
+
 int evaluate(gern_pipeline p, size_t variant, const char *who, void *stream, const std::map<std::string, void *> &args) {
     try {
         Runner *runner = p->variants[variant].runner.get();
@@ -107,15 +114,14 @@ bool aligned(const void *pointer, uintptr_t bytes) {
     return reinterpret_cast<uintptr_t>(pointer) % bytes == 0;
 }
 
+struct Buffer {
+    const void *at;
+    int64_t bytes;
+};
+
 // A launch has less than 2^32 threads along x.
 bool tooWide(int64_t workgroups, int64_t threads) {
     return workgroups * threads > 0xffffffff;
-}
-
-// Whether [a, a + na) and [b, b + nb), sizes in bytes, share memory.
-bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
-    const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-    return na > 0 && nb > 0 && pa < pb + (uintptr_t)nb && pb < pa + (uintptr_t)na;
 }
 
 bool goodPageSize(int64_t page_size) {
@@ -197,10 +203,6 @@ int gern_page_table_run(gern_pipeline p, const int32_t *cached, const int32_t *a
         (tokens > 0 && slots == nullptr) || (free_capacity > 0 && free_pages == nullptr)) {
         return fail("gern_page_table_run: null buffer");
     }
-    struct Buffer {
-        const void *at;
-        int64_t bytes;
-    };
     const Buffer in[] = {{cached, 4 * requests}, {added, 4 * requests}, {free_pages, 4 * free_capacity}, {free_count, 4}};
     const Buffer results[] = {{table, 4 * requests * table_width}, {lengths, 4 * requests}, {starts, 4 * (requests + 1)}, {slots, 4 * tokens}, {counts, 8}};
     for (const auto &b : in) {
@@ -251,6 +253,15 @@ std::string cacheProblem(const void *k_cache, const void *v_cache, const float *
         return "pages must be at least 1, and pages * page_size less than 2^31";
     }
     return "";
+}
+
+struct CacheBuffers {
+    Buffer codes[2], scales[2];
+};
+CacheBuffers cacheBuffers(gern_pipeline p, const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales, int64_t pages,
+                          int64_t heads) {
+    const int64_t scales = pages * heads * (int64_t)sizeof(float), codes = pages * heads * p->page_size * p->head_dim;
+    return {{{k_cache, codes}, {v_cache, codes}}, {{k_scales, scales}, {v_scales, scales}}};
 }
 
 }  // namespace
@@ -327,6 +338,22 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
     }
     if (tooWide(pieces, single ? 64 : 256)) {
         return fail("gern_cache_write_run: tokens / page_size * heads must be less than 2^23");
+    }
+    if (!compileOnly(p)) {
+        const CacheBuffers buffers = cacheBuffers(p, k_cache, v_cache, k_scales, v_scales, pages, heads);
+        const Buffer results[] = {buffers.codes[0], buffers.codes[1], buffers.scales[0], buffers.scales[1]};
+        const int64_t width = heads * p->head_dim * 2;
+        for (const auto &r : results) {
+            if (overlap(Rows{K, tokens, ldk * 2, width}, r.at, r.bytes) || overlap(Rows{V, tokens, ldv * 2, width}, r.at, r.bytes) ||
+                overlap(slots, 4 * tokens, r.at, r.bytes)) {
+                return fail("gern_cache_write_run: K, V or the slots share memory with the cache");
+            }
+            for (const auto &other : results) {
+                if (&other != &r && overlap(r.at, r.bytes, other.at, other.bytes)) {
+                    return fail("gern_cache_write_run: codes or scales of keys and of values share memory");
+                }
+            }
+        }
     }
     hip::WritableCache cache{{k_cache, v_cache, k_scales, v_scales, pages, heads, p->fault_count}, pieces, stretch};
     return evaluate(p, single ? 0 : 1, "gern_cache_write_run", stream, {{"tokens", &fresh}, {"cache", &cache}});
@@ -541,8 +568,26 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     if (needed > 0 && tooWide(join_blocks, 256)) {
         return fail("gern_cache_attention_run: tokens * q_heads must be less than 2^24 where keys are split into more than 16 pieces, 2^26 into fewer");
     }
-    if (needed > 0 && overlap(workspace, needed, O, ((tokens - 1) * ldo + q_heads * p->head_dim) * 2)) {
+    const Rows q{Q, tokens, ldq * 2, q_heads * p->head_dim * 2}, o{O, tokens, ldo * 2, q_heads * p->head_dim * 2};
+    if (needed > 0 && overlap(o, workspace, needed)) {
         return fail("gern_cache_attention_run: the workspace shares memory with O");
+    }
+    if (!compileOnly(p)) {
+        const CacheBuffers buffers = cacheBuffers(p, k_cache, v_cache, k_scales, v_scales, pages, heads);
+        const Buffer in[] = {buffers.codes[0], buffers.codes[1], buffers.scales[0], buffers.scales[1], {table, 4 * requests * table_width},
+                             {lengths, 4 * requests}, {starts, 4 * (requests + 1)}};
+        const bool in_place = Q == O && (ldq == ldo || tokens == 1);
+        if (!in_place && overlap(q, o)) {
+            return fail("gern_cache_attention_run: O shares memory with Q and is not in its place");
+        }
+        if (needed > 0 && overlap(q, workspace, needed)) {
+            return fail("gern_cache_attention_run: the workspace shares memory with Q");
+        }
+        for (const auto &b : in) {
+            if (overlap(o, b.at, b.bytes) || overlap(workspace, needed, b.at, b.bytes)) {
+                return fail("gern_cache_attention_run: O or the workspace shares memory with the cache, the table, lengths or starts");
+            }
+        }
     }
     float *partial = static_cast<float *>(workspace), *stats = needed > 0 ? partial + plan.splits * rows * p->head_dim : nullptr;
     hip::AttentionBatch batch{Q, ldq / 2, table, lengths, starts, table_width, tokens, group, scale * 1.4426950408889634f};

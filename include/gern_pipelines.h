@@ -230,7 +230,8 @@ int gern_page_table_run(gern_pipeline p, const int32_t *cached, const int32_t *a
  * Tokens of one page must be consecutive and in order in a call (as
  * gern_page_table_run makes them): the page's tokens in front of the first one
  * are kept, and what stands behind the last one is unspecified.  Two such runs
- * of tokens for one page in one call race on that page. */
+ * of tokens for one page in one call race on that page.  The four arrays of the
+ * cache share memory neither with one another nor with K, V and slots. */
 int gern_cache_write_create(int64_t head_dim, int64_t page_size, int type, int flags, gern_pipeline *out);
 int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void *V, int64_t ldv,
                          const int32_t *slots, int64_t tokens, int64_t heads, uint8_t *k_cache,
@@ -245,7 +246,8 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  *   O = softmax(scale * q . k) v over the keys a query sees, 0 where it sees none
  * (a request of length 0, a query in front of the first key), in `type`, row
  * stride ldo; rows of Q in no request are left alone in O.  O may be Q (with the
- * same stride); it shares memory with nothing else that the call reads.
+ * same stride), or stand beside it in the same rows; it shares memory with
+ * nothing else that the call reads, and neither does the workspace.
  * max_queries and max_length tell the most queries and keys of one request; the
  * division of the work and the workspace depend on them, results only in their
  * rounding (more are computed, too, only slower).  A weight (a value's share
