@@ -4,6 +4,8 @@
 
 #include "annot/pieces.h"
 
+#include <cstddef>
+
 namespace gern {
 namespace hip {
 
@@ -19,6 +21,11 @@ struct MatvecOut {
     void *y;
     int64_t pitch, columns;
 };
+
+// The sizes and last members' places that csrc/gernel_check.hip asks of gernels::.
+static_assert(sizeof(Activations) == 24 && offsetof(Activations, rows) == 16);
+static_assert(sizeof(Weights4) == 40 && offsetof(Weights4, k) == 32);
+static_assert(sizeof(MatvecOut) == 24 && offsetof(MatvecOut, columns) == 16);
 
 }  // namespace hip
 }  // namespace gern

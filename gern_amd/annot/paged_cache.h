@@ -5,6 +5,8 @@
 
 #include "annot/pieces.h"
 
+#include <cstddef>
+
 namespace gern {
 namespace hip {
 
@@ -57,6 +59,17 @@ struct JoinRows {
     const int32_t *starts;
     int64_t splits, requests, q_heads, rows, blocks;
 };
+
+// The sizes and last members' places that csrc/gernel_check.hip asks of gernels::.
+static_assert(sizeof(PagedCache) == 56 && offsetof(PagedCache, faults) == 48);
+static_assert(sizeof(WritableCache) == 72);
+static_assert(sizeof(NewTokens) == 48 && offsetof(NewTokens, tokens) == 40);
+static_assert(sizeof(RequestLengths) == 24 && offsetof(RequestLengths, requests) == 16);
+static_assert(sizeof(FreePages) == 24 && offsetof(FreePages, capacity) == 16);
+static_assert(sizeof(PageTableOut) == 64 && offsetof(PageTableOut, shares) == 56);
+static_assert(sizeof(AttentionBatch) == 72 && offsetof(AttentionBatch, scale) == 64);
+static_assert(sizeof(AttentionOut) == 72 && offsetof(AttentionOut, requests) == 64);
+static_assert(sizeof(JoinRows) == 80 && offsetof(JoinRows, blocks) == 72);
 
 }  // namespace hip
 

@@ -216,3 +216,19 @@ template __global__ void check_matvec4<128, 1, 1, gernels::Bf16>(gernels::Activa
 template __global__ void check_matvec4<64, 1, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
 template __global__ void check_matvec4<64, 2, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
 template __global__ void check_matvec4<32, 4, 4, gernels::F16>(gernels::ActivationsOf<gernels::F16>, gernels::Weights4, gernels::MatvecOut);
+
+// The layouts of what the host hands to these gernels (annot/paged_cache.h, annot/matvec4.h ask the same of its mirrors).
+namespace gernels {
+static_assert(sizeof(PagedCache) == 56 && offsetof(PagedCache, faults) == 48);
+static_assert(sizeof(WritableCache) == 72);
+static_assert(sizeof(NewTokensOf<Bf16>) == 48 && offsetof(NewTokensOf<Bf16>, tokens) == 40);
+static_assert(sizeof(RequestLengths) == 24 && offsetof(RequestLengths, requests) == 16);
+static_assert(sizeof(FreePages) == 24 && offsetof(FreePages, capacity) == 16);
+static_assert(sizeof(PageTableOut) == 64 && offsetof(PageTableOut, shares) == 56);
+static_assert(sizeof(AttentionBatchOf<F16>) == 72 && offsetof(AttentionBatchOf<F16>, scale) == 64);
+static_assert(sizeof(AttentionOut) == 72 && offsetof(AttentionOut, requests) == 64);
+static_assert(sizeof(JoinRows) == 80 && offsetof(JoinRows, blocks) == 72);
+static_assert(sizeof(ActivationsOf<F16>) == 24 && offsetof(ActivationsOf<F16>, rows) == 16);
+static_assert(sizeof(Weights4) == 40 && offsetof(Weights4, k) == 32);
+static_assert(sizeof(MatvecOut) == 24 && offsetof(MatvecOut, columns) == 16);
+}  // namespace gernels
