@@ -367,6 +367,7 @@ namespace {
 struct AttentionPlan {
     size_t variant;
     int64_t row_tiles, splits, chunk;
+    bool whole_will_do;  // workgroups are enough without a split
 };
 
 constexpr int64_t kMaxSplits = 256;  // gernels/serving/cache_attention.h, join_splits
@@ -410,7 +411,17 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
     // 2000: 16.0, 12.1), nor are workgroups for every CU four times over (128 requests of 1000 to 2000, 8 heads
     // of 128: 87 whole, 97 in two).  Pieces of 256 / 512 / 1024 at least: 16 requests of 2000 to 4000 33.3 / 31.7 / 27.5, one
     // of 32768 18.4 / 17.1 / 19.5, two of 20000, 4 heads 16.0 / 15.8 / 18.6.
-    const int64_t splits = max_length <= 1024 || whole >= 1024 ? 1 : std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
+    int64_t splits = max_length <= 1024 || whole >= 1024 ? 1 : std::clamp<int64_t>((wanted + whole - 1) / whole, 1, kMaxSplits);
+    // But a request that is far longer than the others must not be what all wait for: few rows in workgroups enough are
+    // divided into pieces of 4096 keys, as long as the parts of `rows` queries a request take no more than 256 MiB.  Whole /
+    // pieces of 2048 / 4096 / 8192 (us, 8 heads of 128): 127 requests of 4000 to 8000 and one of 262144 3176 / 737 / 730 /
+    // 809, one of 20000 388 / 322 / 315 / 345; 128 of 2000 to 4000 153 / 158 / - / -, of 4096 to 8192 312 / 302 / 294 / -,
+    // of 16384 to 32768 1182 / 1112 / 1086 / 1088.
+    plan.whole_will_do = plan.variant == kFewRows && whole >= 1024;
+    if (plan.whole_will_do) {
+        const int64_t part = requests * heads * rows * (head_dim + 2) * (int64_t)sizeof(float);
+        splits = std::clamp<int64_t>(std::min<int64_t>((max_length + 4095) / 4096, (256 << 20) / part), 1, kMaxSplits);
+    }
     // Undivided keys, and a CU for every workgroup: its wavefronts' steps of 32 keys one after the other are what a call
     // takes, so there are twice as many.  8 heads of 128, us with 4 / 8 wavefronts: 1 request of 1000 keys 11.3 / 10.3, 32 of
     // 1000 15.1 / 13.7 (of 256: 23.6 / 23.8); 1 of 500 9.4 / 9.5 (of 256: 10.1 / 10.4); 64 of 1000, two workgroups a CU, 24 / 26.
@@ -557,8 +568,12 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
         return fail("gern_cache_attention_run: a row stride is less than q_heads * head_dim");
     }
     const int64_t group = q_heads / heads;
-    const AttentionPlan plan = attentionPlan(p->head_dim, requests, heads, max_queries * group, max_length);
-    const int64_t needed = attentionWorkspace(plan, tokens, q_heads, p->head_dim);
+    AttentionPlan plan = attentionPlan(p->head_dim, requests, heads, max_queries * group, max_length);
+    int64_t needed = attentionWorkspace(plan, tokens, q_heads, p->head_dim);
+    if (plan.whole_will_do && (workspace == nullptr || workspace_bytes < needed)) {
+        plan.splits = 1;
+        needed = 0;
+    }
     if (needed > 0 && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 16))) {
         return fail("gern_cache_attention_run: the workspace must be 16-byte aligned and hold the " + std::to_string(needed) +
                     " bytes that gern_cache_attention_workspace says");

@@ -52,11 +52,11 @@ class Request:
         self.k, self.v, self.vs = E4M3[kc] * of[0][:, None], E4M3[vc] * of[1][:, None], of[1]
 
     def run(self, torch, gpu, scale, few=True, splits=True):
-        """The result.  `few`: the program for few rows.  Not `splits`: as among 1024 workgroups, whose keys are not divided (requests
-        without tokens, or room for more queries)."""
+        """The result.  `few`: the program for few rows.  Not `splits`: as among so many workgroups that keys are not divided (requests
+        without tokens and room for 64 rows each, whose parts would take too much memory, or room for more queries)."""
         queries, heads, dim = self.q.shape
-        requests = 1 if splits or not few else 1024
-        max_queries = queries if few else 100 if splits else 1 << 17
+        requests = 1 if splits or not few or self.length <= 1024 else 16384
+        max_queries = (queries if requests == 1 else 64 // heads) if few else 100 if splits else 1 << 17
         a = gpu("CacheAttention", head_dim=dim, page_size=self.page, dtype=self.dtype)
         n = a.workspace_bytes(queries, requests, heads, 1, max_queries, self.length)
         assert (n > 0) == splits
@@ -82,7 +82,7 @@ class Request:
 def test_attention_keeps_small_weights(torch, gpu, few, splits, length, above, ratio, spread):  # noqa: F811
     """One key far above the others, whose value is 0 in most dimensions, on a page of a larger scale: what the others add up
     to there is the result."""
-    dim, page, queries = 64, 16, 2 if few else 100
+    dim, page, queries = 64, 128 if few and not splits else 16, 2 if few else 100
     rs = np.random.RandomState(length + above)
     q = rs.normal(size=(queries, 2, dim))
     q[..., 0] = 1.0
