@@ -329,7 +329,9 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
     }
     hip::NewTokens fresh{K, V, ldk / 2, ldv / 2, slots, tokens};
     // One token per workgroup of one wavefront while that gives no more workgroups than the GPU runs at a time;
-    // beyond that a page's worth of tokens per workgroup of four.
+    // beyond that a page's worth of tokens per workgroup of four.  us, 8 heads of 128, one / the other: 256 requests of one
+    // token, pages of 16 8.4 / 18, of 128 8.5 / 183; 1024 requests 9.9 / 25, 11.5 / 183; a prompt of 8192 tokens 15.4 / 8.3,
+    // 31 / 8.3.  A prompt of 1024 tokens, 8.5 / 8.6 and 16.2 / 8.4, looks like 1024 requests from here.
     const bool single = tokens * heads * 2 <= 16384;
     const int64_t stretch = single ? 1 : p->page_size;
     const int64_t pieces = (tokens + stretch - 1) / stretch * heads * 2;
@@ -394,14 +396,19 @@ int attentionResidentWaves(int64_t head_dim) {
 
 AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, int64_t rows, int64_t max_length) {
     AttentionPlan plan{};
-    // 32 requests of 2000 to 4000 keys, 8 heads of 128, us with few / many rows a program: 16 rows 56 / 91, 32 rows 63 / 93,
-    // 64 rows 91 / 101.
+    // us with the program for few / many rows: 32 requests of 2000 to 4000 keys, 8 heads, 16 rows of 64 dimensions 30 / 62, of
+    // 128 44 / 93, of 192 60 / 103, of 256 91 / 114; 64 rows 59 / 68, 95 / 102, 117 / 116, 164 / 130; 96 rows 60 / 77, 100 / 113,
+    // 113 / 153, 153 / 168; 128 rows 81 / 78, 121 / 115, 157 / 162, 205 / 177.  4 requests of 500 to 1000, 64 rows: 10 / 29,
+    // 12 / 40, - , 18 / 41.
     plan.variant = rows <= 64 ? kFewRows : kManyRows;
     const int64_t tile = plan.variant == kFewRows ? 16 : 16 * kAttentionPrograms[kManyRows].waves * attentionRowTiles(head_dim);
     plan.row_tiles = std::max<int64_t>(1, (rows + tile - 1) / tile);
     // Keys are split, into pieces of at least 512, until there are `wanted` workgroups.  Eight for each of 256 CUs: two
     // to three times what is resident, so that requests of different lengths leave few CUs idle at the end.  Few rows of
-    // more than 128 dimensions: two, what is resident, because the joined parts are larger and a start costs more.
+    // more than 128 dimensions: two, what is resident, because the joined parts are larger and a start costs more (32
+    // requests of 2000 to 4000 keys, 8 heads, one query, with 512 / 1024 / 2048: of 64 dimensions 28 / 26 / 28, of 128
+    // 38 / 44 / 42, of 192 56 / 58 / 64, of 256 89 / 87 / 92; 2 of 65536 to 131072: 48 / 43 / 40, 84 / 77 / 79,
+    // 114 / 121 / 116, 150 / 156 / 149).
     // Measured (us) with 512 / 1024 / 2048 / 4096: 64 requests of 4096 to 8192 keys, 8 heads of 128: 181 / 175 / 155 /
     // 165; 3 of 131072 to 262144: 266 / 188 / 184 / 197; 32 of 1250 to 2500, 16 heads of 256: 95 / 110 / 109 / -; 6 of 113
     // to 447 queries and 4032 to 5915 keys, 4 heads of 64 for 16: - / 103 / 97 / 103.
@@ -423,8 +430,9 @@ AttentionPlan attentionPlan(int64_t head_dim, int64_t requests, int64_t heads, i
         splits = std::clamp<int64_t>(std::min<int64_t>((max_length + 4095) / 4096, (256 << 20) / part), 1, kMaxSplits);
     }
     // Undivided keys, and a CU for every workgroup: its wavefronts' steps of 32 keys one after the other are what a call
-    // takes, so there are twice as many.  8 heads of 128, us with 4 / 8 wavefronts: 1 request of 1000 keys 11.3 / 10.3, 32 of
-    // 1000 15.1 / 13.7 (of 256: 23.6 / 23.8); 1 of 500 9.4 / 9.5 (of 256: 10.1 / 10.4); 64 of 1000, two workgroups a CU, 24 / 26.
+    // takes, so there are twice as many.  8 heads of 64, 128, 192, 256, us with 4 / 8 wavefronts: 1 request of 500 to 1000
+    // keys 10.6 / 10.2, 12.3 / 10.9, 13.8 / 12.4, 16.7 / 16.0; 32 11.4 / 10.2, 15.5 / 13.9, 18.7 / 17.7, 21.8 / 23.5; 1 of 250 to
+    // 500 10.6 / 10.5, 10.2 / 10.3, 10.1 / 10.1, 11.3 / 11.6; 64 of 1000, 128, two workgroups a CU, 24 / 26.
     if (plan.variant == kFewRows && max_length > 512 && max_length <= 1024 && whole <= 256) {
         plan.variant = kFewRowsWide;
     }
@@ -578,6 +586,8 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
         return fail("gern_cache_attention_run: the workspace must be 16-byte aligned and hold the " + std::to_string(needed) +
                     " bytes that gern_cache_attention_workspace says");
     }
+    // one query, 8 heads of 128, us with a wavefront / a workgroup a row: 8 splits 13.7 / 13.6, 16 13.7 / 14.1, 32 13.9 / 14.6,
+    // 63 19.0 / 17.4; 300 queries, 14 splits 97 / 101
     const bool wave_a_row = plan.splits <= 16;
     const int64_t rows = tokens * q_heads, join_blocks = wave_a_row ? (rows + 3) / 4 : rows;
     if (needed > 0 && tooWide(join_blocks, 256)) {
@@ -630,7 +640,8 @@ struct MatvecShape {
 constexpr MatvecShape kMatvecShapes[] = {{0, 1}, {0, 2}, {0, 4}, {1, 1}, {1, 2}, {1, 3}, {1, 4}, {2, 1}, {2, 4}, {4, 1}, {4, 4}};
 constexpr int64_t kMatvecWaves = 8;
 
-// The program for M rows and N columns: the one whose slowest CU has least to do.  A workgroup's work is its tiles of
+// The program for M rows and N columns: the one whose slowest CU has least to do, with a workgroup a CU at a time (more
+// fit, and share what it can do).  A workgroup's work is its tiles of
 // columns, and what it does for x whatever their number: as much as 0.7 of a tile with up to 4 rows, as 2 tiles for
 // every 16 rows beyond that.  Measured (us, K = 8192 but where said), one to four tiles of columns:
 //   1 row:   28672 columns 33 / 31 / 31 / 30, 16384 of K = 4096 9.7 / 9.8 / - / 9.2, 8192 11.3 / 9.7 / - / 12.5

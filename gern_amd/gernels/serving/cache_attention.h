@@ -38,7 +38,7 @@
 // they add up to.)  o <= 2^15 * 448 * 2^30 keys is far from the end of fp32.
 //
 // Bound by memory for few queries: 2 D bytes a key and head, read once (64 requests of
-// 4096 to 8192 keys, 8 heads of 128: 788 MB in 155 us, 5.1 TB/s; a copy of 1 GiB
+// 4096 to 8192 keys, 8 heads of 128: 788 MB in 154 us, 5.1 TB/s; a copy of 1 GiB
 // moves 5.2 on the same GPU).
 #pragma once
 
@@ -452,7 +452,7 @@ struct AttentionRequest {
 // row that does not see the key) and put into the results of the rows that do when all are stored.  This does so for the rows
 // [row, end) and the `count` keys at begin + offset, + step ... of their split: with `all` for all of them, which does no harm,
 // or for those that the first row does not see.  It is rare, and reads the codes again: noted in the loop over the keys, or
-// done right behind it, it would cost every call of few rows (64 requests: 177 and 160 us for 155).
+// done right behind it, it would cost every call of few rows (64 requests: 177 and 160 us for 154).
 template<int D, int PAGE, class T>
 __device__ __forceinline__ void return_nan(const AttentionRequest<D, PAGE, T> &request, const AttentionPiece &piece, const KeyWalk<D, PAGE> &walk, int row,
                                            int end, int offset, int count, int step, bool all) {
@@ -661,10 +661,12 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
 // instructions take, a 16-key tile by each wavefront: codes are converted and
 // values transposed once for the whole workgroup, and fragments are read 16 bytes
 // a lane without bank conflicts.  The next block's codes are loaded while this one
-// is multiplied.  Bound by the vector ALU: per 16 rows and 32 keys a softmax of 8
-// scores a lane (8 exponentials at a quarter of the rate) stands against D / 8 matrix
-// instructions.  6 requests of 113 to 447 queries and 4032 to 5915 keys, 16 heads of
-// 64 on 4: 30.6 GFLOP in 101 us, 15 of them the join of six splits (213 us with keys
+// is multiplied.  Per 16 rows and 32 keys a softmax of 8 scores a lane (8
+// exponentials at a quarter of the rate) stands against D / 8 matrix instructions, but
+// what bounds it are waits: 1.6 wavefronts a SIMD between barriers, a third of whose time
+// is waiting, keep the vector ALU busy for 45 % of the time and the matrix cores for
+// 13 %.  6 requests of 113 to 447 queries and 4032 to 5915 keys, 16 heads of
+// 64 on 4: 30.6 GFLOP in 100 us, 15 of them the join of six splits (213 us with keys
 // from memory for every wavefront).
 template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, class T>
 __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {

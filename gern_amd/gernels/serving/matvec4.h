@@ -23,10 +23,11 @@
 // result's size against the 2^-8 (bf16) or 2^-11 (fp16) of its last rounding.
 //
 // The wavefronts of a workgroup divide K and add their sums in LDS, in a fixed
-// order.  Measured: 1 row, 28672 columns, K = 8192, G = 128 in 27.6 us (4.5 TB/s of
+// order.  Measured: 1 row, 28672 columns, K = 8192, G = 128 in 27.5 us (4.5 TB/s of
 // codes, scales and zero points; a copy of 1 GiB moves 5.2 on the same GPU); 13
-// rows, 10001 columns, K = 8192, G = 64 in 15.6 us (2.9 TB/s: bound by the vector
-// ALU, which takes 7 instructions for 8 codes and 8 for the sums of a group).
+// rows, 10001 columns, K = 8192, G = 64 in 15.6 us (2.9 TB/s: bound by the latency
+// of its loads, a block ahead for one wavefront a SIMD on 209 CUs; the vector ALU is
+// busy for 24 % of the time, the matrix cores for 6 %).
 #pragma once
 
 #include "gernels/serving/half_tiles.h"

@@ -288,8 +288,9 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
  * divides K, which is at most GERN_MATVEC4_MAX_COLUMNS.  Sums
  * are fp32, rounded once; those of bf16 are taken of 2^-16 of the products, so
  * that no finite X overflows on the way, and X under 2^-116 keeps fewer bits.
- * A row of X with an infinity gives NaN.  For more rows the products, and no longer the weights, are the work:
- * that is gern_gemm_run's. */
+ * A row of X with an infinity gives NaN.  More rows are several calls, of which
+ * each reads the weights; products of many rows with bf16 weights are
+ * gern_gemm_run's. */
 #define GERN_MATVEC4_MAX_ROWS 64
 #define GERN_MATVEC4_MAX_COLUMNS (1 << 24)
 int gern_matvec4_create(int64_t group, int type, int flags, gern_pipeline *out);
