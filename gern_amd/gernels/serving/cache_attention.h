@@ -69,7 +69,7 @@ struct AttentionOut {
     uint32_t *out;       // two values a word
     int64_t out_pitch;   // words
     float *partial;      // [splits, tokens * query heads, D], with splits > 1
-    float *stats;        // [splits, tokens * query heads, 2]: maximum less kWeightBits, sum
+    float *stats;        // [splits, tokens * query heads, 2]: taken off the exponents, sum
     int64_t splits;      // of the keys, `chunk` each (the last one takes the rest)
     int64_t chunk;
     int64_t pieces;      // workgroups per request and head: row tiles * splits
@@ -133,6 +133,12 @@ constexpr float kLowest = -1.0e30f;
 
 // log2 of a row's largest weight: the largest power of two of fp16.
 constexpr float kWeightBits = 15.0f;
+// What is taken off the exponents of a row with this maximum: the maximum less kWeightBits, or the maximum itself where
+// (from 2^24 on) the difference is rounded down and a weight would leave fp16.
+__device__ __forceinline__ float less_weight_bits(float most) {
+    const float less = most - kWeightBits;
+    return most - less > kWeightBits ? most : less;
+}
 
 // The least scale of values, 2^-80: 2^30 weights of 2^15, each over it, add up to less than 2^126.  What is under it
 // counts as 0: the softmax takes it as this, and the values are 0.
@@ -213,11 +219,9 @@ struct TileScales {
 };
 template<int D>
 __device__ __forceinline__ TileScales scales_of(const RawKeys<D> &tile, float scale) {
-    // The scale of the scores stays above zero because -infinity, a key that is not seen, is multiplied by it: at 2^-126 a
-    // score is 0 but for products of queries and codes beyond 2^100.
-    const float k = tile.k_scale * scale, v = tile.v_scale;
+    const float v = tile.v_scale;
     const float vs = !tile.there ? 1.0f : v < kLeastValueScale ? kLeastValueScale : v;
-    return {!tile.there ? 1.0f : k < 1.17549435e-38f ? 1.17549435e-38f : k, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
+    return {tile.k_scale * scale, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), tile.there};
 }
 
 // What a wavefront needs to walk the keys of one request and head.
@@ -266,7 +270,7 @@ template<int D, int R, bool BF16>
 struct RowState {
     Frag q[R][D / 32];     // lane (g, c): row c, dimensions g D/4 + 8 s ..
     f32x4 o[R][D / 16];    // lane (g, c): row c, o[.][i][e] is dimension (4 g + e) D/16 + i
-    float m[R], l[R];      // maximum over the row less kWeightBits, sum over this lane's keys
+    float m[R], l[R];      // taken off the row's exponents (less_weight_bits), sum over this lane's keys
     int limit[R];          // keys that row c sees
 
     __device__ __forceinline__ void clear() {
@@ -310,9 +314,24 @@ struct RowState {
             scales[t] = scales_of_tile(t);
         }
         after_keys();
+        // Many rows one after the other: of 64 dimensions 32 bytes a lane are spilled otherwise (prompt pieces 101.5 us, 115.8
+        // without), of 128 and 192 it is faster (300 queries 117 / 120, 161 / 175 us); of 256 it is not (199 / 188), nor with few rows.
+        constexpr bool kInTurn = PAIRS > 1 && D <= 192;
+        if constexpr (kInTurn) {
+            __builtin_amdgcn_sched_barrier(0);
+        }
         Frag p[R][PAIRS];
 #pragma unroll
         for (int r = 0; r < R; r++) {
+            // A score is rounded once, before the maximum is taken and before it is subtracted: however large scores are, the
+            // largest one's weight is what it should be.  (In one step, s k + (up - m), it would be off by m's rounding.)
+#pragma unroll
+            for (int t = 0; t < kTiles; t++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[r][t][e] = __builtin_fmaf(s[r][t][e], scales[t].k, scales[t].up);
+                }
+            }
             if (!whole) {
 #pragma unroll
                 for (int t = 0; t < kTiles; t++) {
@@ -323,17 +342,16 @@ struct RowState {
                     }
                 }
             }
-            // scales are not negative: the largest product of a tile is its largest score
             float top = kLowest;
 #pragma unroll
             for (int t = 0; t < kTiles; t++) {
-                const float most = larger(larger(s[r][t][0], s[r][t][1]), larger(s[r][t][2], s[r][t][3]));
-                const float score = __builtin_fmaf(most, scales[t].k, scales[t].up);
+                const float score = larger(larger(s[r][t][0], s[r][t][1]), larger(s[r][t][2], s[r][t][3]));
                 top = t == 0 ? score : larger(top, score);
             }
-            top = max_over_lane_groups(top) - kWeightBits;
-            if (__ballot(top > m[r]) != 0) {
-                const float now = larger(top, m[r]);
+            top = max_over_lane_groups(top);
+            const bool more = top - m[r] > kWeightBits;
+            if (__ballot(more) != 0) {
+                const float now = more ? less_weight_bits(top) : m[r];
                 const float shrink = __builtin_amdgcn_exp2f(m[r] - now);
                 m[r] = now;
                 l[r] *= shrink;
@@ -344,15 +362,17 @@ struct RowState {
             }
 #pragma unroll
             for (int t = 0; t < kTiles; t++) {
-                const float shift = scales[t].up - m[r];
                 float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    y[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][t][e], scales[t].k, shift));
+                    y[e] = __builtin_amdgcn_exp2f(s[r][t][e] - m[r]);
                     l[r] = __builtin_fmaf(y[e], scales[t].per_v, l[r]);
                 }
                 p[r][t / 2].w[2 * (t % 2)] = pack_halves<F16>(y[0], y[1]);
                 p[r][t / 2].w[2 * (t % 2) + 1] = pack_halves<F16>(y[2], y[3]);
+            }
+            if constexpr (kInTurn) {
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll

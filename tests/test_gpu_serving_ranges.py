@@ -214,3 +214,38 @@ def test_matvec_small_activations(torch, gpu, m, group):  # noqa: F811
     # where the group is added; all times 2^16
     steps = 2.0 ** -150 * (4 * (8 + group / 32) + 1) * scales.double().numpy().sum(axis=0) * 2.0 ** 16
     assert np.all(np.abs(y.double().cpu().numpy() - want) <= tol + steps + HALF_STEP["bf16"] * (np.abs(want) + tol + steps))
+
+
+@pytest.mark.parametrize("few, length, splits", [(True, 300, False), (True, 5000, True), (False, 300, False), (False, 5000, True)])
+@pytest.mark.parametrize("power", [10, 18, 20, 22, 24, 26, 30, 50, 90])
+def test_attention_large_scores(torch, gpu, few, length, splits, power):  # noqa: F811
+    """Scores of both signs up to 2^98: with gaps beyond what 32 bits leave between them, a query's result is its best key's value."""
+    dim, page, queries = 64, 16, 2 if few else 90
+    rs = np.random.RandomState(power)
+    k = np.zeros((length, dim))
+    k[:, 0] = rs.randint(-8, 8, length) + 0.5  # ties share the row
+    k[:, 1] = rs.choice([-0.5, 0.0, 0.5], length)
+    q = np.zeros((queries, 2, dim))
+    q[..., 0], q[..., 1] = 2.0 ** power * rs.choice([-1.25, 1.0, 1.5], (queries, 2)), 2.0 ** (power - 3)
+    pages = -(-length // page)
+    r = Request(torch, "bf16", page, code_of(k), code_of(rs.normal(size=(length, dim)) * 16), np.full(pages, 16.0), 1.37 * np.exp2(rs.randint(-9, 4, pages)), q)
+    out = r.run(torch, gpu, 1.0, few, splits)
+    for h in range(2):
+        q = r.q[:, h].double().numpy()
+        for i in range(queries):
+            n = length - queries + i + 1
+            z = r.k[:n] @ q[i]
+            best = z == z.max()
+            assert np.sort(z[~best])[-1] < z.max() - 200.0  # nothing else has a weight
+            want = r.v[:n][best].mean(axis=0)
+            # the best keys' scores are equal, and so are their exponents but for their scales' logarithms, which are added in 32 bits
+            step = 2.0 ** -24 * (np.abs(z.max()) * 1.4427 + 16)
+            if best.sum() == 1 or step < 2.0 ** -6:
+                size = np.abs(r.v[:n][best]).mean(axis=0)
+                tol = (2.0 ** -11 + (8 * step if best.sum() > 1 else 0.0) + 2.0 ** -18) * size
+                assert np.all(np.abs(out[i, h] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol)), (i, h)
+            else:
+                # weights of ties are off by the rounding of their exponents: the result is between the ties' values
+                lo, hi = r.v[:n][best].min(axis=0), r.v[:n][best].max(axis=0)
+                slack = HALF_STEP["bf16"] * np.maximum(np.abs(lo), np.abs(hi)) * 1.01
+                assert np.all(out[i, h] >= lo - slack) and np.all(out[i, h] <= hi + slack), (i, h)
