@@ -578,7 +578,7 @@ int gern_cache_attention_run(gern_pipeline p, const void *Q, int64_t ldq, const 
     const int64_t group = q_heads / heads;
     AttentionPlan plan = attentionPlan(p->head_dim, requests, heads, max_queries * group, max_length);
     int64_t needed = attentionWorkspace(plan, tokens, q_heads, p->head_dim);
-    if (plan.whole_will_do && (workspace == nullptr || workspace_bytes < needed)) {
+    if (plan.whole_will_do && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 16))) {
         plan.splits = 1;
         needed = 0;
     }

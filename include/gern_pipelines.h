@@ -257,7 +257,7 @@ int gern_cache_write_run(gern_pipeline p, const void *K, int64_t ldk, const void
  * call's from its launch to its end: calls that overlap in time need one each.
  * One launch, or two where the keys are split among workgroups.  A large batch
  * of few queries each (1024 workgroups and more) runs undivided, too, with less
- * workspace or none, but waits for its longest request then.
+ * workspace, none or an unaligned one, but waits for its longest request then.
  * Keys on a page that is not in the cache (a table entry outside [0, pages), or
  * lengths[r] beyond the table) are left out, and gern_pipeline_faults is not 0
  * then.  What stands behind the last key, in its page or in the table, is not

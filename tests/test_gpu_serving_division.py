@@ -20,7 +20,8 @@ def test_one_long_request_of_many(torch, gpu, dim, heads, group, queries):  # no
     tokens, scale = device["q"].shape[0], dim ** -0.5
     n = a.workspace_bytes(tokens, requests, heads * group, heads, queries, 9000)
     assert n == 3 * tokens * heads * group * (dim + 2) * 4  # pieces of 3072 keys
-    for workspace in (torch.full((n,), 255, dtype=torch.uint8, device="cuda"), None, torch.empty(n - 16, dtype=torch.uint8, device="cuda")):
+    for workspace in (torch.full((n,), 255, dtype=torch.uint8, device="cuda"), None, torch.empty(n - 16, dtype=torch.uint8, device="cuda"),
+                      torch.empty(n + 8, dtype=torch.uint8, device="cuda")[8:]):
         out.fill_(77.0)
         a(**device, scale=scale, max_queries=queries, max_length=9000, workspace=workspace)
         torch.cuda.synchronize()
