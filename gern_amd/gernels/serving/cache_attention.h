@@ -133,11 +133,13 @@ constexpr float kLowest = -1.0e30f;
 
 // log2 of a row's largest weight: the largest power of two of fp16.
 constexpr float kWeightBits = 15.0f;
-// What is taken off the exponents of a row with this maximum: the maximum less kWeightBits, or the maximum itself where
-// (from 2^24 on) the difference is rounded down and a weight would leave fp16.
+// What is taken off the exponents of a row with this maximum: the maximum less kWeightBits, so that its own weight is a
+// power of two and not rounded; or the maximum itself where (from 2^24 on) the difference is rounded down and a weight would
+// leave fp16.  (Differences of ordinary scores are off by 2^-20: that is not more.)
+constexpr float kMoreThanWeightBits = 15.001f;
 __device__ __forceinline__ float less_weight_bits(float most) {
     const float less = most - kWeightBits;
-    return most - less > kWeightBits ? most : less;
+    return most - less > kMoreThanWeightBits ? most : less;
 }
 
 // The least scale of values, 2^-80: 2^30 weights of 2^15, each over it, add up to less than 2^126.  What is under it
@@ -349,7 +351,7 @@ struct RowState {
                 top = t == 0 ? score : larger(top, score);
             }
             top = max_over_lane_groups(top);
-            const bool more = top - m[r] > kWeightBits;
+            const bool more = top - m[r] > kMoreThanWeightBits;
             if (__ballot(more) != 0) {
                 const float now = more ? less_weight_bits(top) : m[r];
                 const float shrink = __builtin_amdgcn_exp2f(m[r] - now);
