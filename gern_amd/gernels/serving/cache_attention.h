@@ -686,9 +686,9 @@ __device__ __forceinline__ void attend_few_rows(const AttentionBatchOf<T> &batch
 // is multiplied.  Per 16 rows and 32 keys a softmax of 8 scores a lane (8
 // exponentials at a quarter of the rate) stands against D / 8 matrix instructions, but
 // what bounds it are waits: 1.6 wavefronts a SIMD between barriers, a third of whose time
-// is waiting, keep the vector ALU busy for 45 % of the time and the matrix cores for
+// is waiting, keep the vector ALU busy for 47 % of the time and the matrix cores for
 // 13 %.  6 requests of 113 to 447 queries and 4032 to 5915 keys, 16 heads of
-// 64 on 4: 30.6 GFLOP in 100 us, 15 of them the join of six splits (213 us with keys
+// 64 on 4: 30.6 GFLOP in 101 us, 15 of them the join of six splits (213 us with keys
 // from memory for every wavefront).
 template<int64_t D, int64_t PAGE, int64_t R, int64_t WAVES, class T>
 __device__ __forceinline__ void attend_many_rows(const AttentionBatchOf<T> &batch, const PagedCache &cache, const AttentionPiece &piece) {

