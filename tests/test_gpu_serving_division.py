@@ -1,9 +1,9 @@
-"""Attention over the cache of a large batch with a request that is far longer than the others."""
+"""Attention over the cache of batches whose requests differ much, and of more queries than a call says."""
 import numpy as np
 import pytest
 
 import serving_oracle as so
-from test_gpu_serving import HALF_STEP, attention_inputs, gpu, torch  # noqa: F401  (fixtures)
+from test_gpu_serving import HALF_STEP, attention_inputs, check_attention, gpu, run_attention, torch  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,23 @@ def test_one_long_request_of_many(torch, gpu, dim, heads, group, queries):  # no
                 for u in range(h * group, (h + 1) * group):
                     want, tol = so.attention(host["q"][starts[b]:starts[b] + m, u], k, v, vs, length - m + np.arange(m) + 1, scale)
                     assert np.all(np.abs(o[starts[b]:starts[b] + m, u] - want) <= tol + HALF_STEP["bf16"] * (np.abs(want) + tol)), (b, u)
+
+
+@pytest.mark.parametrize("dim, group", [(64, 1), (128, 2), (192, 1), (256, 1)])
+def test_whole_prompts(torch, gpu, dim, group):  # noqa: F811
+    """As many queries as keys: the first one sees one key."""
+    run_attention(torch, gpu, "bf16", dim, 32, 1, group, [400, 1, 257, 0], [400, 1, 257, 0], seed=dim)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("length, said", [(600, 1), (600, 70), (3000, 1), (3000, 70)])
+def test_more_queries_and_keys_than_said(torch, gpu, dim, length, said):  # noqa: F811
+    """Workgroups of either program that take rows after rows, the keys undivided and divided."""
+    device, host, out = attention_inputs(torch, "f16", dim, 16, 1, 1, [length, 300], [300, 2], seed=length + dim)
+    a = gpu("CacheAttention", head_dim=dim, page_size=16, dtype="f16")
+    n = a.workspace_bytes(device["q"].shape[0], 2, 1, 1, said, length // 2 + 300)
+    for _ in range(2):  # the second run finds the first one's parts
+        a(**device, scale=dim ** -0.5, max_queries=said, max_length=length // 2 + 300, workspace=torch.empty(n, dtype=torch.uint8, device="cuda"))
+        torch.cuda.synchronize()
+        assert a.faults() == 0 and (n > 0) == (length > 1500)
+        check_attention(out, host, "f16", 16, 1, dim ** -0.5)
